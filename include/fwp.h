@@ -108,7 +108,8 @@ unsigned long long fwp_launch_count(void);
  * sequence per SM, four beyond), 6 for the delta rule at sizes up to 32 and at E up to 96 with M up to 32; any of the three keeps the
  * general form where it is not asked for),
  * "delta_bwd.phases" (-1 automatic / 1 / 0: the three-launch backward over scratch, see below), "delta_bwd.32.tile" (1 / 0: the
- * fp32 backward at E = M = 32 step by step over four warps a sequence, or the four-step blocked kernel).  Returns 0 if accepted, FWP_ERR_UNSUPPORTED for an unknown key. */
+ * fp32 backward at E = M = 32 step by step over four warps a sequence, or the four-step blocked kernel),
+ * "scan.chunk" (0 automatic; n: the selective scan works on spans of n steps, rounded up to whole tiles, side by side).  Returns 0 if accepted, FWP_ERR_UNSUPPORTED for an unknown key. */
 int fwp_tune(const char* key, int value);
 /* Name of the kernel this host thread launched last through the library ("" before the
  * first launch): lets a benchmark label its numbers with the plan the dispatch picked. */
@@ -394,6 +395,73 @@ int fwp_fast_lstm_backward_from_outputs(int variant, int N, int H, int L, int D,
                            const fwp_tensor grad_Z[3], const fwp_tensor grad_K[3],
                            const fwp_tensor grad_V[3], const fwp_tensor grad_beta[3],
                            int io_dtype, void* stream, int device);
+
+/* ---- operators of a state-space layer --------------------------------------
+ * No counterpart in the reference.  Streams are (N, L, D) tensors: the descriptor's stride[0] is the sequence's, stride[2] the
+ * step's, stride[1] is not read.  B and C are (N, G, L, S) in the descriptor's order.  Weights are fp32 and contiguous.
+ * `lengths` (int32, one per sequence, on the device; may be NULL): steps at or beyond a sequence's length are not read and their
+ * outputs and gradients are zero; values are taken between 0 and L.  N, L, D may be 0: nothing is read or written then.
+ * States are fp32, in/out in the forwards.  The backwards neither read nor rewind them: a state that decays cannot be run
+ * backwards, so they start from what the forward kept (`start`, `checkpoints`).  No gradient reaches a state.
+ * Scratch and checkpoints are the caller's, 16-byte aligned, contents undefined before.
+ *
+ * Short causal convolution per channel, K taps (1 <= K <= 8):
+ *   p_t = bias + sum_j weight[d, j] x_{t-K+1+j},  out_t = silu ? p_t sigmoid(p_t) : p_t
+ * state [N,1,K-1,D]: the last K-1 inputs, oldest first; may be NULL or have data == NULL (zeros before the first step). */
+int fwp_causal_conv_forward(int N, int L, int D, int K, const fwp_tensor* x, const float* weight, const float* bias,
+                            const fwp_tensor* state, const int* lengths, const fwp_tensor* out, int silu,
+                            int io_dtype, void* stream, int device);
+/* start: the state as it was before the forward, never written. grad_weight [D,K]; grad_bias [D] or NULL. */
+int64_t fwp_causal_conv_backward_scratch_floats(int N, int L, int D, int K);
+int fwp_causal_conv_backward(int N, int L, int D, int K, const fwp_tensor* x, const float* weight, const float* bias,
+                             const fwp_tensor* start, const int* lengths, const fwp_tensor* grad_out, const fwp_tensor* grad_x,
+                             float* grad_weight, float* grad_bias, float* scratch, int64_t scratch_floats, int silu,
+                             int io_dtype, void* stream, int device);
+
+/* Selective scan, S <= 64 states per channel, G groups of D / G channels that share B and C:
+ *   delta = softplus ? log(1 + exp(dt + dt_bias)) : dt + dt_bias
+ *   h_t = exp(delta_t A) h_{t-1} + delta_t x_t B_t,   y_t = C_t h_t + skip x_t,   out_t = z ? y_t z_t sigmoid(z_t) : y_t
+ * A [D,S]; skip, dt_bias [D] or NULL; z may have data == NULL; state [N,1,D,S] or NULL (h_{-1} = 0).
+ * checkpoints (may be NULL when no backward follows): fwp_selective_scan_checkpoint_floats(...) floats, the state before every
+ * eighth step.  Scratch: fwp_selective_scan_scratch_floats(...) floats for long sequences over few channels, 0 for others. */
+int64_t fwp_selective_scan_checkpoint_floats(int N, int L, int D, int S);
+int64_t fwp_selective_scan_scratch_floats(int N, int L, int D, int S, int G, int device);
+int fwp_selective_scan_forward(int N, int L, int D, int S, int G, const fwp_tensor* x, const fwp_tensor* dt, const float* A,
+                               const fwp_tensor* B, const fwp_tensor* C, const float* skip, const fwp_tensor* z,
+                               const float* dt_bias, const fwp_tensor* state, const int* lengths, const fwp_tensor* out,
+                               float* checkpoints, float* scratch, int64_t scratch_floats, int softplus,
+                               int io_dtype, void* stream, int device);
+/* grad_A [D,S]; grad_skip, grad_dt_bias [D] (NULL where the input is); grad_B, grad_C [N,G,L,S] like B and C. */
+int64_t fwp_selective_scan_backward_scratch_floats(int N, int L, int D, int S, int G, int device);
+int fwp_selective_scan_backward(int N, int L, int D, int S, int G, const fwp_tensor* x, const fwp_tensor* dt, const float* A,
+                                const fwp_tensor* B, const fwp_tensor* C, const float* skip, const fwp_tensor* z,
+                                const float* dt_bias, const int* lengths, const float* checkpoints, const fwp_tensor* grad_out,
+                                const fwp_tensor* grad_x, const fwp_tensor* grad_dt, float* grad_A, const fwp_tensor* grad_B,
+                                const fwp_tensor* grad_C, float* grad_skip, const fwp_tensor* grad_z, float* grad_dt_bias,
+                                float* scratch, int64_t scratch_floats, int softplus, int io_dtype, void* stream, int device);
+
+/* What stands between two blocks: the norm behind a block, its gate and residual scale, the residual sum and the norm before
+ * the next block.  Rows of D <= 8192 elements, N x L of them:
+ *   t = post_weight ? norm(x; post_weight, post_bias) : x,   u = gate ? t act(gate) : t
+ *   r = residual + scale u,   y = norm(r; weight, bias)
+ *   norm(v; w, b) = (v - mean v) / sqrt(var v + eps) w + b,  with rms: v / sqrt(mean v^2 + eps) w
+ * gate_act 0: act(g) = g silu-wise (g sigmoid(g)), 1: sigmoid(g), 2: g.  scale: scale_vector [D], or the number scale_value where
+ * that is NULL.  residual, gate: data == NULL for none.  y has x's element type; residual and r have residual_dtype, which is
+ * io_dtype or FWP_F32.  stats (may be NULL when no backward follows): N*L*4 floats. */
+int fwp_block_norm_forward(int N, int L, int D, const fwp_tensor* x, const fwp_tensor* residual, const fwp_tensor* gate,
+                           const float* scale_vector, float scale_value, const float* post_weight, const float* post_bias,
+                           const float* weight, const float* bias, const fwp_tensor* y, const fwp_tensor* r, float* stats,
+                           float eps, int rms, int gate_act, int io_dtype, int residual_dtype, void* stream, int device);
+/* grad_y, grad_r: data == NULL counts as zeros.  grad_x, grad_gate have io_dtype, grad_residual residual_dtype (data == NULL:
+ * not wanted); vector gradients [D] fp32, NULL where the input is. */
+int64_t fwp_block_norm_backward_scratch_floats(int N, int L, int D);
+int fwp_block_norm_backward(int N, int L, int D, const fwp_tensor* x, const fwp_tensor* residual, const fwp_tensor* gate,
+                            const float* scale_vector, float scale_value, const float* post_weight, const float* post_bias,
+                            const float* weight, const float* bias, const float* stats, const fwp_tensor* grad_y,
+                            const fwp_tensor* grad_r, const fwp_tensor* grad_x, const fwp_tensor* grad_residual,
+                            const fwp_tensor* grad_gate, float* grad_scale, float* grad_post_weight, float* grad_post_bias,
+                            float* grad_weight, float* grad_bias, float* scratch, int64_t scratch_floats, int rms, int gate_act,
+                            int io_dtype, int residual_dtype, void* stream, int device);
 
 #ifdef __cplusplus
 }

@@ -18,6 +18,9 @@ from .fast_lstm import FastLSTM, fast_lstm  # noqa: F401
 from .fast_lstm_v2 import FastLSTMv2, fast_lstm_v2  # noqa: F401
 from .fast_lstm_v3 import FastLSTMv3, fast_lstm_v3  # noqa: F401
 from .fast_lstm_v4 import FastLSTMv4, fast_lstm_v4  # noqa: F401
+from .causal_conv import causal_conv  # noqa: F401
+from .selective_scan import selective_scan  # noqa: F401
+from .block_norm import block_norm  # noqa: F401
 
 __all__ = ['DeltaFastWeight', 'fast_weight_delta', 'FastWeightSum', 'fast_weight_sum',
            'FastWeightRecUpdateTanh', 'rec_update_fwm_tanh', 'FastRNNv2', 'fast_rnn_v2', 'FastRNN', 'fast_rnn',

@@ -44,6 +44,7 @@ native = _load_native()
 _T = ctypes.POINTER(FwpTensor)
 _T3 = ctypes.POINTER(FwpTensor)   # arrays of three descriptors are passed as pointers
 _i, _vp, _i64 = ctypes.c_int, ctypes.c_void_p, ctypes.c_int64
+_fl = ctypes.c_float
 
 # name -> argument types, exactly as declared in include/fwp.h
 SIGNATURES = {
@@ -70,11 +71,21 @@ SIGNATURES = {
     'fwp_debug_bounded_wait_probe': [_i, _vp, _i],
     'fwp_delayed': [_i] * 4 + [_T] * 4 + [_i, _vp, _i],
     'fwp_fast_lstm_backward': [_i] * 5 + [_T] + [_T3] * 4 + [_T] * 4 + [_T3] * 6 + [_i, _vp, _i],
+    # weights, lengths, workspaces and vector gradients are passed as plain device addresses
+    'fwp_causal_conv_forward': [_i] * 4 + [_T, _vp, _vp, _T, _vp, _T, _i] + [_i, _vp, _i],
+    'fwp_causal_conv_backward': [_i] * 4 + [_T, _vp, _vp, _T, _vp, _T, _T, _vp, _vp, _vp, _i64, _i] + [_i, _vp, _i],
+    'fwp_selective_scan_forward': [_i] * 5 + [_T, _T, _vp, _T, _T, _vp, _T, _vp, _T, _vp, _T, _vp, _vp, _i64, _i] + [_i, _vp, _i],
+    'fwp_selective_scan_backward': [_i] * 5 + [_T, _T, _vp, _T, _T, _vp, _T, _vp, _vp, _vp, _T, _T, _T, _vp, _T, _T, _vp, _T, _vp,
+                                               _vp, _i64, _i] + [_i, _vp, _i],
+    'fwp_block_norm_forward': [_i] * 3 + [_T] * 3 + [_vp, _fl] + [_vp] * 4 + [_T, _T, _vp, _fl, _i, _i, _i] + [_i, _vp, _i],
+    'fwp_block_norm_backward': [_i] * 3 + [_T] * 3 + [_vp, _fl] + [_vp] * 5 + [_T] * 5 + [_vp] * 6 + [_i64, _i, _i, _i] + [_i, _vp, _i],
     'fwp_fast_lstm_backward_from_outputs': [_i] * 5 + [_T] + [_T3] * 4 + [_T] * 4 + [_T3] * 6 + [_i, _vp, _i],
 }
 OTHER_SYMBOLS = ['fwp_status_string', 'fwp_last_cuda_error', 'fwp_version', 'fwp_max_head_dim',
                  'fwp_launch_count', 'fwp_tune', 'fwp_rec_update_fwm_tanh_scratch_floats', 'fwp_delta_device_fault',
-                 'fwp_last_kernel', 'fwp_fast_weight_backward_scratch_floats']
+                 'fwp_last_kernel', 'fwp_fast_weight_backward_scratch_floats', 'fwp_causal_conv_backward_scratch_floats',
+                 'fwp_selective_scan_checkpoint_floats', 'fwp_selective_scan_scratch_floats',
+                 'fwp_selective_scan_backward_scratch_floats', 'fwp_block_norm_backward_scratch_floats']
 
 for _name, _args in SIGNATURES.items():
     _f = getattr(lib, _name)
@@ -89,6 +100,11 @@ lib.fwp_rec_update_fwm_tanh_scratch_floats.restype = _i64
 lib.fwp_fast_weight_backward_scratch_floats.argtypes = [_i] * 6
 lib.fwp_fast_weight_backward_scratch_floats.restype = _i64
 lib.fwp_last_kernel.restype = ctypes.c_char_p
+for _name, _n in (('fwp_causal_conv_backward_scratch_floats', 4), ('fwp_selective_scan_checkpoint_floats', 4),
+                  ('fwp_selective_scan_scratch_floats', 6), ('fwp_selective_scan_backward_scratch_floats', 6),
+                  ('fwp_block_norm_backward_scratch_floats', 3)):
+    getattr(lib, _name).argtypes = [_i] * _n
+    getattr(lib, _name).restype = _i64
 
 
 def io_dtype(t):
@@ -184,6 +200,29 @@ def unit_inner(t):
     if t.shape[-1] == 1 or t.stride(-1) == 1:
         return t
     return t.contiguous()
+
+
+def sequence_lengths(ref, lengths, n):
+    """Lengths of a padded batch as the kernels read them: int32 on the streams' device, or None."""
+    if lengths is None:
+        return None
+    if lengths.dtype not in (torch.int32, torch.int64):
+        raise TypeError('lengths must be int32 or int64, got %s' % lengths.dtype)
+    if lengths.device != ref.device or tuple(lengths.shape) != (n,):
+        raise RuntimeError('lengths is %s on %s, expected (%d,) on %s' % (tuple(lengths.shape), lengths.device, n, ref.device))
+    if lengths.dtype == torch.int64:
+        lengths = lengths.clamp(0, 2 ** 31 - 1).to(torch.int32)
+    return lengths.contiguous()
+
+
+def require_state(state):
+    """A state that a kernel updates in place."""
+    if state is None:
+        return
+    if state.shape[-1] > 1 and state.stride(-1) != 1:
+        raise RuntimeError('state must have a unit innermost stride (it is updated in place)')
+    if any(n > 1 and s == 0 for n, s in zip(state.shape, state.stride())):
+        raise RuntimeError('state must not be an expanded tensor (it is updated in place)')
 
 
 class _Recorded(torch.autograd.Function):

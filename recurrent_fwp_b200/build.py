@@ -62,7 +62,7 @@ def _binding_stamp():
 
 
 def _binding_stale():
-    if _newer([BINDING_SRC] + glob.glob(os.path.join(PKG, '..', 'include', '*.h')), BINDING):
+    if _newer([BINDING_SRC] + glob.glob(os.path.join(CSRC, 'binding', '*.h')) + glob.glob(os.path.join(PKG, '..', 'include', '*.h')), BINDING):
         return True
     try:
         with open(BINDING_STAMP) as f:

@@ -599,6 +599,8 @@ PyObject* fast_lstm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+#include "fwp_torch_blocks.h"
+
 PyObject* check_device_fault(PyObject*, PyObject* on) {
     g_check_fault = PyObject_IsTrue(on) == 1;
     Py_RETURN_NONE;
@@ -616,6 +618,9 @@ PyMethodDef methods[] = {
     OP("fast_lstm_v2", fast_lstm<2>),
     OP("fast_lstm_v3", fast_lstm<3>),
     OP("fast_lstm_v4", fast_lstm<4>),
+    OP("causal_conv", causal_conv),
+    OP("selective_scan", selective_scan),
+    OP("block_norm", block_norm),
     {"check_device_fault", check_device_fault, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

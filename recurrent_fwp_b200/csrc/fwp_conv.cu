@@ -1,0 +1,355 @@
+// Short causal convolution per channel (sm_100a), forward and backward.
+//
+//   p_t = bias + sum_j w_j x_{t-K+1+j},  out_t = p_t sigmoid(p_t)
+//   gp_t = gout_t silu'(p_t),  gx_t = sum_j w_j gp_{t+K-1-j},  gw_j = sum_t gp_t x_{t-K+1+j}
+//
+// Bound by the bytes: forward one element in and one out per (n, t, d), backward two in and one out.  A warp owns 32 x V channels
+// of one sequence and walks a span of steps with the last K - 1 inputs in registers, so every input is read once (and K - 1 of
+// a neighbour's span, from L2); eight rows are in flight per warp.  The backward walks forwards too: it forms p again from
+// the inputs it needs for gw anyway, and gx K - 1 steps behind.
+#include "fwp_seq.cuh"
+
+namespace fwp {
+
+constexpr int kConvMaxK = 8;
+constexpr int kConvWarps = 4;
+constexpr int kConvRows = 8;            // rows loaded ahead of their use
+
+struct ConvParams {
+    Stream x, state, out, gout, gx;     // state: rows are the K - 1 inputs before the first
+    const float *w, *b;
+    const int* lengths;
+    float* part;                        // backward: [N * span groups][D * (K + 1)]
+    int N, L, D, silu, span, spans, groups;     // groups: of 32 x V channels
+};
+
+template <int K, int V>
+__device__ __forceinline__ void conv_weights(const ConvParams& p, int d0, int nd, float (&w)[K][V], float (&b)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        b[i] = i < nd && p.b ? p.b[d0 + i] : 0.f;
+#pragma unroll
+        for (int j = 0; j < K; j++) w[j][i] = i < nd ? p.w[(long long)(d0 + i) * K + j] : 0.f;
+    }
+}
+
+// the K - 1 inputs before step t0 (steps below zero come from the state, or are zero)
+template <typename T, int K, int V>
+__device__ __forceinline__ void conv_window(const ConvParams& p, const T* x, int n, int t0, int d0, float (&win)[K][V]) {
+#pragma unroll
+    for (int j = 0; j < K - 1; j++) {
+        const int t = t0 - (K - 1) + j;
+#pragma unroll
+        for (int i = 0; i < V; i++) win[j][i] = 0.f;
+        if (t >= 0) load_vec<V>(x + t * p.x.sL, win[j]);
+        else if (p.state.p)
+            load_vec<V>(static_cast<const float*>(p.state.p) + n * p.state.sN + (long long)(t + K - 1) * p.state.sL + d0, win[j]);
+    }
+}
+
+template <typename T, int K, int V>
+__global__ void __launch_bounds__(kConvWarps * 32) conv_fwd_kernel(ConvParams p) {
+    griddep_wait();
+    griddep_launch_dependents();
+    const int lane = threadIdx.x & 31, n = blockIdx.z;
+    const int d0 = (blockIdx.x * 32 + lane) * V;
+    const int s = blockIdx.y * kConvWarps + (threadIdx.x >> 5);
+    if (d0 >= p.D || s >= p.spans) return;
+    const int len = p.lengths ? min(max(p.lengths[n], 0), p.L) : p.L;
+    const int t0 = s * p.span, t1 = min(t0 + p.span, len), tend = min(t0 + p.span, p.L);
+    const T* x = static_cast<const T*>(p.x.p) + n * p.x.sN + d0;
+    T* out = static_cast<T*>(p.out.p) + n * p.out.sN + d0;
+    float w[K][V], b[V], win[K][V];
+    if (t0 < t1 || s == 0) {
+        conv_weights<K, V>(p, d0, V, w, b);
+        conv_window<T, K, V>(p, x, n, t0, d0, win);
+    }
+    // the first span reads the state before the steps, and writes the one behind them: nobody else touches it
+    if (s == 0 && p.state.p && K > 1) {
+        float* st = static_cast<float*>(p.state.p) + n * p.state.sN + d0;
+        float end[K][V];
+#pragma unroll
+        for (int j = 0; j < K - 1; j++) {
+            const int t = len - (K - 1) + j;
+#pragma unroll
+            for (int i = 0; i < V; i++) end[j][i] = 0.f;
+            if (t >= 0) load_vec<V>(x + t * p.x.sL, end[j]);
+            else {
+                // input t lies in the old state, at row t + K - 1
+#pragma unroll
+                for (int q = 0; q < K - 1; q++)
+                    if (q == t + K - 1) {
+#pragma unroll
+                        for (int i = 0; i < V; i++) end[j][i] = win[q][i];
+                    }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < K - 1; j++) store_vec<V>(st + j * p.state.sL, end[j]);
+    }
+    for (int t = t0; t < t1; t += kConvRows) {
+        float in[kConvRows][V];
+#pragma unroll
+        for (int r = 0; r < kConvRows; r++) {
+#pragma unroll
+            for (int i = 0; i < V; i++) in[r][i] = 0.f;
+            if (t + r < t1) load_vec<V>(x + (long long)(t + r) * p.x.sL, in[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < kConvRows; r++) {
+            float y[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                win[K - 1][i] = in[r][i];
+                float a = b[i];
+#pragma unroll
+                for (int j = 0; j < K; j++) a = fmaf(w[j][i], win[j][i], a);
+                y[i] = p.silu ? a * sigmoidf_(a) : a;
+#pragma unroll
+                for (int j = 0; j < K - 1; j++) win[j][i] = win[j + 1][i];
+            }
+            if (t + r < t1) store_vec<V>(out + (long long)(t + r) * p.out.sL, y);
+        }
+    }
+    const float zero[V] = {};
+    for (int t = max(t0, t1); t < tend; t++) store_vec<V>(out + (long long)t * p.out.sL, zero);
+}
+
+template <typename T, int K, int V>
+__global__ void __launch_bounds__(kConvWarps * 32) conv_bwd_kernel(ConvParams p) {
+    __shared__ float red[kConvWarps][K + 1][32 * V];
+    griddep_wait();
+    griddep_launch_dependents();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockIdx.z;
+    const int d0 = (blockIdx.x * 32 + lane) * V;
+    const int s = blockIdx.y * kConvWarps + warp;
+    const bool on = d0 < p.D && s < p.spans;
+    float gw[K][V], gb[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        gb[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < K; j++) gw[j][i] = 0.f;
+    }
+    if (on) {
+        const int len = p.lengths ? min(max(p.lengths[n], 0), p.L) : p.L;
+        const int t0 = s * p.span, t1 = min(t0 + p.span, len), tend = min(t0 + p.span, p.L);
+        const T* x = static_cast<const T*>(p.x.p) + n * p.x.sN + d0;
+        const T* gout = static_cast<const T*>(p.gout.p) + n * p.gout.sN + d0;
+        T* gx = static_cast<T*>(p.gx.p) + n * p.gx.sN + d0;
+        if (t0 < t1) {
+            float w[K][V], b[V], win[K][V], gp[K][V];      // gp[j]: of step u - K + 1 + j
+            conv_weights<K, V>(p, d0, V, w, b);
+            conv_window<T, K, V>(p, x, n, t0, d0, win);
+#pragma unroll
+            for (int j = 0; j < K; j++)
+#pragma unroll
+                for (int i = 0; i < V; i++) gp[j][i] = 0.f;
+            const int uend = t1 + K - 1;                   // steps from t1 on belong to the next span: only their gp counts here
+            for (int u0 = t0; u0 < uend; u0 += kConvRows) {
+                float in[kConvRows][V], go[kConvRows][V];
+#pragma unroll
+                for (int r = 0; r < kConvRows; r++) {
+#pragma unroll
+                    for (int i = 0; i < V; i++) in[r][i] = go[r][i] = 0.f;
+                    if (u0 + r < min(uend, len)) {
+                        load_vec<V>(x + (long long)(u0 + r) * p.x.sL, in[r]);
+                        load_vec<V>(gout + (long long)(u0 + r) * p.gout.sL, go[r]);
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < kConvRows; r++) {
+                    const int u = u0 + r;
+                    float g[V];
+#pragma unroll
+                    for (int i = 0; i < V; i++) {
+                        win[K - 1][i] = in[r][i];
+                        float a = b[i];
+#pragma unroll
+                        for (int j = 0; j < K; j++) a = fmaf(w[j][i], win[j][i], a);
+                        float d = go[r][i];
+                        if (p.silu) d *= silu_grad_of(a, sigmoidf_(a));
+                        d = u < len ? d : 0.f;
+                        gp[K - 1][i] = d;
+                        if (u < t1) {
+                            gb[i] += d;
+#pragma unroll
+                            for (int j = 0; j < K; j++) gw[j][i] = fmaf(d, win[j][i], gw[j][i]);
+                        }
+                        float q = 0.f;
+#pragma unroll
+                        for (int j = 0; j < K; j++) q = fmaf(w[j][i], gp[K - 1 - j][i], q);     // gp of step (u - K + 1) + K - 1 - j
+                        g[i] = q;
+#pragma unroll
+                        for (int j = 0; j < K - 1; j++) { win[j][i] = win[j + 1][i]; gp[j][i] = gp[j + 1][i]; }
+                    }
+                    const int t = u - (K - 1);
+                    if (t >= t0 && t < t1) store_vec<V>(gx + (long long)t * p.gx.sL, g);
+                }
+            }
+        }
+        const float zero[V] = {};
+        for (int t = max(t0, t1); t < tend; t++) store_vec<V>(gx + (long long)t * p.gx.sL, zero);
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        red[warp][K][lane * V + i] = gb[i];
+#pragma unroll
+        for (int j = 0; j < K; j++) red[warp][j][lane * V + i] = gw[j][i];
+    }
+    __syncthreads();
+    // partial sums of the CTA: weights as [D][K], then the bias
+    float* part = p.part + ((long long)n * gridDim.y + blockIdx.y) * p.D * (K + 1);
+    for (int i = threadIdx.x; i < 32 * V * (K + 1); i += kConvWarps * 32) {
+        const int j = i / (32 * V), c = i - j * (32 * V), d = blockIdx.x * 32 * V + c;
+        if (d >= p.D) continue;
+        float a = 0.f;
+#pragma unroll
+        for (int q = 0; q < kConvWarps; q++) a += red[q][j][c];
+        part[j == K ? (long long)p.D * K + d : (long long)d * K + j] = a;
+    }
+}
+
+// Steps a warp walks: long spans read fewer neighbours' steps, short ones fill the machine when there are few channels.
+static int conv_span(int N, int L, int D, int V) {
+    const long long columns = (long long)N * ceil_div(D, 32 * V), sms = sm_count() > 0 ? sm_count() : 148;
+    int span = 64;
+    while (span > kConvRows && columns * ceil_div(L, span) < sms * 16) span >>= 1;
+    while (ceil_div(L, (long long)span * kConvWarps) > 65535) span <<= 1;      // the grid's limit
+    return span;
+}
+
+static int conv_check(int N, int L, int D, int K, const fwp_tensor* x, const float* w, const float* b, const fwp_tensor* state,
+                      const int* lengths, int io_dtype) {
+    if (N < 0 || L < 0 || D < 0 || K < 1) return FWP_ERR_SHAPE;
+    if (io_dtype != FWP_F32 && io_dtype != FWP_BF16) return FWP_ERR_DTYPE;
+    if (K > kConvMaxK) return FWP_ERR_UNSUPPORTED;
+    if (N > 65535) return FWP_ERR_SHAPE;
+    if (D && !w) return FWP_ERR_NULL;
+    if (!aligned4(w) || !aligned4(b) || !aligned4(lengths)) return FWP_ERR_ALIGN;
+    if (!N || !L || !D) return FWP_OK;
+    if (int rc = check_tensor(x, io_dtype == FWP_F32 ? 4 : 2, true)) return rc;
+    return check_tensor(state, 4, false);
+}
+
+static bool conv_vectors(const ConvParams& p, int esz) {
+    return p.D % 4 == 0 && rows_aligned(p.x, esz, 4 * esz) && rows_aligned(p.state, 4, 16) && rows_aligned(p.out, esz, 4 * esz) &&
+           rows_aligned(p.gout, esz, 4 * esz) && rows_aligned(p.gx, esz, 4 * esz);
+}
+
+template <typename T, int K, int V>
+static int conv_launch(ConvParams p, bool backward, cudaStream_t st) {
+    p.span = conv_span(p.N, p.L, p.D, V);
+    p.spans = (int)ceil_div(p.L, p.span);
+    const dim3 grid((unsigned)ceil_div(p.D, 32 * V), (unsigned)ceil_div(p.spans, kConvWarps), (unsigned)p.N);
+    if (backward) return launch_dependent(conv_bwd_kernel<T, K, V>, p, grid, kConvWarps * 32, 0, st, "conv_bwd_kernel");
+    return launch_dependent(conv_fwd_kernel<T, K, V>, p, grid, kConvWarps * 32, 0, st, "conv_fwd_kernel");
+}
+template <typename T, int V>
+static int conv_taps(int K, const ConvParams& p, bool backward, cudaStream_t st) {
+    switch (K) {
+        case 1: return conv_launch<T, 1, V>(p, backward, st);
+        case 2: return conv_launch<T, 2, V>(p, backward, st);
+        case 3: return conv_launch<T, 3, V>(p, backward, st);
+        case 4: return conv_launch<T, 4, V>(p, backward, st);
+        case 5: return conv_launch<T, 5, V>(p, backward, st);
+        case 6: return conv_launch<T, 6, V>(p, backward, st);
+        case 7: return conv_launch<T, 7, V>(p, backward, st);
+    }
+    return conv_launch<T, 8, V>(p, backward, st);
+}
+static int conv_dispatch(int K, const ConvParams& p, bool backward, int io_dtype, cudaStream_t st) {
+    if (io_dtype == FWP_F32) return conv_vectors(p, 4) ? conv_taps<float, 4>(K, p, backward, st) : conv_taps<float, 1>(K, p, backward, st);
+    return conv_vectors(p, 2) ? conv_taps<__nv_bfloat16, 4>(K, p, backward, st) : conv_taps<__nv_bfloat16, 1>(K, p, backward, st);
+}
+
+// rows of partial sums: at most those of the narrowest form
+static long long conv_part_rows(int N, int L, int D) {
+    long long most = 0;
+    for (int V : {1, 4}) {
+        int span = conv_span(N, L, D, V);
+        const long long rows = (long long)N * ceil_div(ceil_div(L, span), kConvWarps);
+        most = rows > most ? rows : most;
+    }
+    return most;
+}
+
+// ---------------------------------------------------------------- sums of partial gradients
+__global__ void __launch_bounds__(256) column_sums_kernel(ColumnSums p) {
+    __shared__ float red[8][33];
+    griddep_wait();
+    griddep_launch_dependents();
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const long long c = (long long)blockIdx.x * 32 + tx;
+    float a = 0.f;
+    if (c < p.W)
+        for (int r = ty; r < p.P; r += 8) a += p.part[r * p.W + c];
+    red[ty][tx] = a;
+    __syncthreads();
+    if (ty || c >= p.W) return;
+#pragma unroll
+    for (int i = 1; i < 8; i++) a += red[i][tx];
+    long long from = 0;
+#pragma unroll
+    for (int k = 0; k < kSumSegments; k++) {
+        if (c >= from && c < p.end[k]) {
+            if (p.out[k]) p.out[k][c - from] = a;
+            return;
+        }
+        from = p.end[k];
+    }
+}
+
+int launch_column_sums(const ColumnSums& p, cudaStream_t st) {
+    return launch_dependent(column_sums_kernel, p, dim3((unsigned)ceil_div(p.W, 32)), 256, 0, st, nullptr);
+}
+
+}  // namespace fwp
+
+using namespace fwp;
+
+FWP_API int fwp_causal_conv_forward(int N, int L, int D, int K, const fwp_tensor* x, const float* weight, const float* bias,
+                                    const fwp_tensor* state, const int* lengths, const fwp_tensor* out, int silu, int io_dtype,
+                                    void* stream, int device) {
+    int rc;
+    if ((rc = conv_check(N, L, D, K, x, weight, bias, state, lengths, io_dtype)) || !N || !L || !D) return rc;
+    if ((rc = check_tensor(out, io_dtype == FWP_F32 ? 4 : 2, true))) return rc;
+    DeviceGuard guard(device);
+    if (guard.status) return guard.status;
+    ConvParams p = {stream_of(x), stream_of(state), stream_of(out), {}, {}, weight, bias, lengths, nullptr, N, L, D, silu ? 1 : 0, 0, 0, 0};
+    return conv_dispatch(K, p, false, io_dtype, (cudaStream_t)stream);
+}
+
+FWP_API int64_t fwp_causal_conv_backward_scratch_floats(int N, int L, int D, int K) {
+    if (N <= 0 || L <= 0 || D <= 0 || K < 1 || K > kConvMaxK) return 0;
+    return conv_part_rows(N, L, D) * D * (K + 1);
+}
+
+FWP_API int fwp_causal_conv_backward(int N, int L, int D, int K, const fwp_tensor* x, const float* weight, const float* bias,
+                                     const fwp_tensor* start, const int* lengths, const fwp_tensor* grad_out, const fwp_tensor* grad_x,
+                                     float* grad_weight, float* grad_bias, float* scratch, int64_t scratch_floats, int silu,
+                                     int io_dtype, void* stream, int device) {
+    const int esz = io_dtype == FWP_F32 ? 4 : 2;
+    int rc;
+    if ((rc = conv_check(N, L, D, K, x, weight, bias, start, lengths, io_dtype))) return rc;
+    if (N && L && D && ((rc = check_tensor(grad_out, esz, true)) || (rc = check_tensor(grad_x, esz, true)))) return rc;
+    if (D && !grad_weight) return FWP_ERR_NULL;
+    if (!aligned4(grad_weight) || !aligned4(grad_bias)) return FWP_ERR_ALIGN;
+    DeviceGuard guard(device);
+    if (guard.status) return guard.status;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (!N || !L || !D) {               // no steps: sums of nothing
+        cudaError_t e = D ? cudaMemsetAsync(grad_weight, 0, sizeof(float) * D * K, st) : cudaSuccess;
+        if (e == cudaSuccess && D && grad_bias) e = cudaMemsetAsync(grad_bias, 0, sizeof(float) * D, st);
+        return e == cudaSuccess ? FWP_OK : set_cuda_error(e);
+    }
+    if (!scratch || !aligned16(scratch) || scratch_floats < fwp_causal_conv_backward_scratch_floats(N, L, D, K)) return FWP_ERR_SCRATCH;
+    ConvParams p = {stream_of(x), stream_of(start), {}, stream_of(grad_out), stream_of(grad_x), weight, bias, lengths, scratch,
+                    N, L, D, silu ? 1 : 0, 0, 0, 0};
+    if ((rc = conv_dispatch(K, p, true, io_dtype, st))) return rc;
+    const int V = conv_vectors(p, esz) ? 4 : 1;
+    const int span = conv_span(N, L, D, V);
+    const long long dk = (long long)D * K;
+    ColumnSums s = {scratch, (int)(N * ceil_div(ceil_div(L, span), kConvWarps)), dk + D, {grad_weight, grad_bias}, {dk, dk + D}};
+    return launch_column_sums(s, st);
+}

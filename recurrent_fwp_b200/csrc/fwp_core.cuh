@@ -69,6 +69,7 @@ enum TuneKey {
     T_DELTA_WY_HELPERS,     // "delta.wy.helpers": 2, 4: preparing warps per sequence of that plan's general form; 4 up to d = 16 and 6 above: its form for few sequences; 0 automatic
     T_DELTA_PHASES,         // "delta_bwd.phases": -1 automatic, 1 / 0 the three-launch backward wherever it has an instance and scratch, or never
     T_DELTA_BWD_TILE32,     // "delta_bwd.32.tile": 1 the backward at E = M = 32 (fp32) step by step over four warps, 0 the blocked kernel
+    T_SCAN_CHUNK,           // "scan.chunk": 0 automatic, n the selective scan takes spans of n steps (rounded up to whole tiles) side by side
     T_COUNT
 };
 int tune_get(TuneKey key, int fallback);

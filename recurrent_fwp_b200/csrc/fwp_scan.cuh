@@ -1,0 +1,136 @@
+// Parameters and device pieces of the selective scan, shared by its forward (fwp_scan.cu) and backward (fwp_scan_bwd.cu).
+#pragma once
+#include "fwp_seq.cuh"
+
+namespace fwp {
+
+constexpr int kScanMaxS = 64;
+// The forward of a call with a backward keeps the state before every eighth step.  The backward then forms exp(delta A) once per
+// state and step, and holds a tile's states and decays in registers; farther apart it would have to form them twice, and the
+// exponentials are what bounds both directions.  8 bytes per (step, channel) each way at S = 16.
+constexpr int kScanKeep = 8;
+
+struct ScanParams {
+    Stream x, dt, z, out;
+    Row4 B, C;              // (N, G, L, S)
+    const float *A, *skip, *dt_bias;
+    const int* lengths;
+    float* state;           // (N, D, S), null: zeros
+    long long state_sN, state_sD;
+    bool state_vec;         // rows of the state move in 16-byte pieces
+    float* checkpoints;     // [N][ceil(L / 8)][D][scan_row(S)]
+    float *ends, *dsums;    // [N][spans][D][S] and [N][spans][D]
+    int N, L, D, S, G, softplus, span, spans;
+    // backward
+    Stream gout, gx, gdt, gz;
+    float *bc, *sums;       // partial gradients of B and C, and of A, skip and dt_bias
+    Row4 gBr, gCr;
+};
+
+// what a pass over the spans of time is for
+enum ScanPass { SCAN_WHOLE = 0, SCAN_ENDS = 1 };
+
+// joins what a pass over the spans left in ends and dsums into the spans' starts; `backwards`: from the last span, which starts from zero
+int launch_scan_join(const ScanParams& p, bool backwards, cudaStream_t st);
+
+// lanes that hold the states of one channel, four each
+static inline int scan_lanes(int S) { return S <= 4 ? 1 : S <= 8 ? 2 : S <= 16 ? 4 : S <= 32 ? 8 : 16; }
+#ifdef __CUDACC__
+__host__ __device__
+#endif
+static inline int scan_row(int S) { return (S + 3) & ~3; }
+
+static inline int scan_check(int N, int L, int D, int S, int G, const fwp_tensor* x, const fwp_tensor* dt, const float* A,
+                             const fwp_tensor* B, const fwp_tensor* C, const float* skip, const fwp_tensor* z, const float* dt_bias,
+                             const int* lengths, int io_dtype) {
+    if (N < 0 || L < 0 || D < 0 || S < 1 || G < 1 || D % G || N > 65535) return FWP_ERR_SHAPE;
+    if (io_dtype != FWP_F32 && io_dtype != FWP_BF16) return FWP_ERR_DTYPE;
+    if (S > kScanMaxS) return FWP_ERR_UNSUPPORTED;
+    if (D && !A) return FWP_ERR_NULL;
+    if (!aligned4(A) || !aligned4(skip) || !aligned4(dt_bias) || !aligned4(lengths)) return FWP_ERR_ALIGN;
+    if (!N || !L || !D) return FWP_OK;
+    const int esz = io_dtype == FWP_F32 ? 4 : 2;
+    int rc;
+    if ((rc = check_tensor(x, esz, true)) || (rc = check_tensor(dt, esz, true)) || (rc = check_tensor(B, esz, true)) ||
+        (rc = check_tensor(C, esz, true)) || (rc = check_tensor(z, esz, false)))
+        return rc;
+    return FWP_OK;
+}
+
+static inline ScanParams scan_params(int N, int L, int D, int S, int G, const fwp_tensor* x, const fwp_tensor* dt, const float* A,
+                                     const fwp_tensor* B, const fwp_tensor* C, const float* skip, const fwp_tensor* z,
+                                     const float* dt_bias, const int* lengths, int softplus) {
+    ScanParams p = {};
+    p.x = stream_of(x); p.dt = stream_of(dt); p.z = stream_of(z);
+    p.B = row4(B); p.C = row4(C);
+    p.A = A; p.skip = skip; p.dt_bias = dt_bias; p.lengths = lengths;
+    p.N = N; p.L = L; p.D = D; p.S = S; p.G = G; p.softplus = softplus ? 1 : 0;
+    return p;
+}
+
+#ifdef __CUDACC__
+
+// log(1 + e^x) with a relative error of a few 1e-7 everywhere.  With e = e^-|x|: max(x, 0) + log(1 + e), and log(1 + e) =
+// 2 atanh(s), s = e / (2 + e) <= 1/3, by its power series to s^15 (the next term is below 1e-9).
+__device__ __forceinline__ float softplus_(float x) {
+    const float e = ex2_approx(-fabsf(x) * kLog2e), s = e * rcp_approx(2.f + e), q = s * s;
+    float r = 1.f / 15.f;
+    r = fmaf(r, q, 1.f / 13.f);
+    r = fmaf(r, q, 1.f / 11.f);
+    r = fmaf(r, q, 1.f / 9.f);
+    r = fmaf(r, q, 1.f / 7.f);
+    r = fmaf(r, q, 1.f / 5.f);
+    r = fmaf(r, q, 1.f / 3.f);
+    r = fmaf(r, q, 1.f);
+    return fmaf(2.f * s, r, x > 0.f ? x : 0.f * x);     // 0 x keeps a NaN
+}
+
+__device__ __forceinline__ f2 exp2_pair(f2 v) {
+    float lo, hi;
+    f2_unpack(v, lo, hi);
+    return f2_pack(ex2_approx(lo), ex2_approx(hi));
+}
+
+// states beyond the last stay zero whatever the streams hold
+__device__ __forceinline__ void keep_states(f2 (&h)[2], int first, int S) {
+    float v[4];
+    f2_unpack(h[0], v[0], v[1]);
+    f2_unpack(h[1], v[2], v[3]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = first + i < S ? v[i] : 0.f;
+    h[0] = f2_pack(v[0], v[1]);
+    h[1] = f2_pack(v[2], v[3]);
+}
+
+template <int CH>
+__device__ __forceinline__ void load_smem(const float* s, float (&v)[CH]) {
+    if constexpr (CH % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < CH; i += 4) {
+            const float4 t = *reinterpret_cast<const float4*>(s + i);
+            v[i] = t.x; v[i + 1] = t.y; v[i + 2] = t.z; v[i + 3] = t.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < CH; i++) v[i] = s[i];
+    }
+}
+
+// the state before step t (a multiple of 8) of the lane's channels
+template <int LPC, int CH>
+__device__ __forceinline__ void scan_checkpoint(const ScanParams& p, int n, int t, int base, int per, int ch0, int j, const f2 (&h)[CH][2]) {
+    const int row = scan_row(p.S);
+    float* at = p.checkpoints + (((long long)n * ((p.L + kScanKeep - 1) / kScanKeep) + t / kScanKeep) * p.D + base) * row + 4 * j;
+    if (4 * j >= row) return;
+#pragma unroll
+    for (int c = 0; c < CH; c++)
+        if (ch0 + c < per) {
+            ulonglong2 v;
+            v.x = h[c][0];
+            v.y = h[c][1];
+            *reinterpret_cast<ulonglong2*>(at + (long long)(ch0 + c) * row) = v;
+        }
+}
+
+#endif
+}  // namespace fwp
