@@ -4,186 +4,169 @@
 //   y_t = sum_s C_t[s] h_t[s] + skip x_t,  out_t = y_t z_t sigmoid(z_t)
 //
 // Every channel is a recurrence of its own over S states, B and C are shared by the channels of a group.  A lane holds four
-// states of CH channels, LPC lanes hold the states of a channel (S <= 4 LPC).  With LPC steps-times-channels in hand the
-// sums over s cost LPC - 1 shuffles and leave each lane with the value of one (step, channel); that lane loads x, dt, z for it
-// and stores its output, so y goes through no memory.
+// states of a channel, LPC lanes a channel (S <= 4 LPC).  With LPC steps in hand the sums over s cost LPC - 1 shuffles and leave each lane
+// with the value of one step; that lane loads x, dt, z for it and stores its output, so y goes through no memory.
 #include "fwp_scan.cuh"
 
 namespace fwp {
 
 constexpr int kScanWarps = 4;
 
-template <typename T, int LPC, int CH>
+template <int LPC>
 struct ScanTile {
-    static constexpr int CW = 32 / LPC * CH;            // channels per warp
-    static constexpr int SP = LPC / CH;                 // steps whose sums are taken together
-    static constexpr int OS = SP <= 4 ? 8 : 32 / SP;    // (step, channel) pairs per lane and tile
-    static constexpr int TT = OS * SP;                  // steps per tile
+    static constexpr int CW = 32 / LPC;                     // channels per warp
+    static constexpr int OS = LPC == 1 ? 8 : LPC <= 4 ? 4 : 16 / LPC;   // (step, channel) pairs per lane and tile
+    static constexpr int TT = OS * LPC;                     // steps per tile
     static constexpr int S4 = 4 * LPC;
-    float delta[kScanWarps][TT][CW];
-    float dx[kScanWarps][TT][CW];
+    float4 st[kScanWarps][TT][CW];                          // delta twice, delta x twice: operands of two-wide products as they are
     float B[2][TT][S4];
     float C[2][TT][S4];
 };
 
 // One span of time of one warp's channels.  PASS = SCAN_ENDS: only the state that the span leaves behind, starting from zero, and
 // the sum of delta, for joining spans (scan_join_kernel).
-template <typename T, int LPC, int CH, bool RAGGED, int PASS>
-__global__ void __launch_bounds__(kScanWarps * 32) scan_fwd_kernel(ScanParams p) {
-    using Tile = ScanTile<T, LPC, CH>;
-    constexpr int CW = Tile::CW, SP = Tile::SP, OS = Tile::OS, TT = Tile::TT, S4 = Tile::S4;
+template <typename T, int LPC, bool RAGGED, int PASS>
+__global__ void __launch_bounds__(kScanWarps * 32, 4) scan_fwd_kernel(ScanParams p) {
+    using Tile = ScanTile<LPC>;
+    constexpr int CW = Tile::CW, OS = Tile::OS, TT = Tile::TT, S4 = Tile::S4, NT = kScanWarps * 32;
+    constexpr bool WHOLE = PASS == SCAN_WHOLE;
     __shared__ __align__(16) Tile sm;
     griddep_wait();
     griddep_launch_dependents();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int grp = lane / LPC, j = lane % LPC;
+    const int grp = lane / LPC, j = lane % LPC;             // channel of the warp; its states 4 j ... 4 j + 3, its steps j, j + LPC ...
     const int n = blockIdx.z, span = blockIdx.y;
     const int per = p.D / p.G, blocks = (per + CW * kScanWarps - 1) / (CW * kScanWarps);
     const int g = blockIdx.x / blocks;
-    const int cw = ((blockIdx.x % blocks) * kScanWarps + warp) * CW;        // first channel of the warp inside the group
+    const int ch = ((blockIdx.x % blocks) * kScanWarps + warp) * CW + grp;      // inside the group
+    const bool on = ch < per;
+    const int d = g * per + (on ? ch : per - 1);            // a lane without a channel reads the last one's rows and writes nothing
     const int len = p.lengths ? min(max(p.lengths[n], 0), p.L) : p.L;
     const int t0 = span * p.span, tend = min(t0 + p.span, p.L), t1 = min(tend, len);
-    // the pair this lane loads and stores: channel `own`, steps so, so + SP, ...
-    const int co = CH * grp + j % CH, so = j / CH;
-    const bool mine = cw + co < per;
-    const int own = g * per + cw + co;
-    const float bias = mine && p.dt_bias ? p.dt_bias[own] : 0.f, skip = mine && p.skip ? p.skip[own] : 0.f;
-    const T* x = static_cast<const T*>(p.x.p) + n * p.x.sN + own;
-    const T* dt = static_cast<const T*>(p.dt.p) + n * p.dt.sN + own;
-    const T* z = static_cast<const T*>(p.z.p) + n * p.z.sN + own;
-    T* out = static_cast<T*>(p.out.p) + n * p.out.sN + own;
+    const float bias = p.dt_bias ? p.dt_bias[d] : 0.f, skip = p.skip ? p.skip[d] : 0.f;
     const bool gated = p.z.p != nullptr;
+    const T* x = static_cast<const T*>(p.x.p) + n * p.x.sN + d;
+    const T* dt = static_cast<const T*>(p.dt.p) + n * p.dt.sN + d;
+    const T* z = static_cast<const T*>(p.z.p) + n * p.z.sN + d;
+    T* out = static_cast<T*>(p.out.p) + n * p.out.sN + d;
 
-    f2 A[CH][2], h[CH][2];
-    const long long spans_at = ((long long)n * p.spans + span) * p.D;       // this span's rows in the workspace
-#pragma unroll
-    for (int c = 0; c < CH; c++) {
-        const int ch = cw + CH * grp + c;
-        const bool on = ch < per;
+    f2 A[2], h[2];
+    const long long spans_at = ((long long)n * p.spans + span) * p.D + d;       // this span's row in the workspace
+    {
         float a[4], s[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int st = 4 * j + i;
-            a[i] = on && st < p.S ? p.A[(long long)(g * per + ch) * p.S + st] * kLog2e : 0.f;
+            a[i] = st < p.S ? p.A[(long long)d * p.S + st] * kLog2e : 0.f;
             s[i] = 0.f;
-            if (PASS == SCAN_WHOLE && on && st < p.S) {
-                if (p.spans > 1) s[i] = p.ends[(spans_at + g * per + ch) * p.S + st];
-                else if (p.state) s[i] = p.state[n * p.state_sN + (g * per + ch) * p.state_sD + st];
+            if (WHOLE && st < p.S) {
+                if (p.spans > 1) s[i] = p.ends[spans_at * p.S + st];
+                else if (p.state) s[i] = p.state[n * p.state_sN + d * p.state_sD + st];
             }
         }
-        A[c][0] = f2_pack(a[0], a[1]); A[c][1] = f2_pack(a[2], a[3]);
-        h[c][0] = f2_pack(s[0], s[1]); h[c][1] = f2_pack(s[2], s[3]);
+        A[0] = f2_pack(a[0], a[1]); A[1] = f2_pack(a[2], a[3]);
+        h[0] = f2_pack(s[0], s[1]); h[1] = f2_pack(s[2], s[3]);
     }
     float dsum = 0.f;
 
-    float rx[OS], rd[OS];                       // the next tile's x and dt
+    // The next tile's streams, as they are in memory: a conversion here would wait for the load.  Rows behind the end repeat the last one.
+    T rx[OS], rd[OS], rz[OS];
+    constexpr int BC = (TT * S4 + NT - 1) / NT;
+    static_assert((TT * S4) % NT == 0 || TT * S4 < NT, "whole passes over a tile of B and C");
+    T rB[BC], rC[BC];
+    const int bc_row = threadIdx.x / S4, bc_s = threadIdx.x % S4;
+    const bool bc_on = (!RAGGED || bc_s < p.S) && bc_row < TT;
+    const T* Bp = static_cast<const T*>(p.B.p) + n * p.B.sN + g * p.B.sH + (bc_on ? bc_s : 0);
+    const T* Cp = static_cast<const T*>(p.C.p) + n * p.C.sN + g * p.C.sH + (bc_on ? bc_s : 0);
     auto fetch = [&](int t) {
 #pragma unroll
         for (int i = 0; i < OS; i++) {
-            const int u = t + so + i * SP;
-            const bool on = mine && u < t1;
-            rx[i] = on ? to_f32(x[u * p.x.sL]) : 0.f;
-            rd[i] = on ? to_f32(dt[u * p.dt.sL]) : 0.f;
+            const int u = min(t + j + i * LPC, t1 - 1);
+            rd[i] = dt[u * p.dt.sL];
+            rx[i] = x[u * p.x.sL];
+            if (WHOLE && gated) rz[i] = z[u * p.z.sL];
         }
-    };
-    constexpr int BC = (TT * S4 + kScanWarps * 32 - 1) / (kScanWarps * 32);
-    float rB[BC], rC[BC];
-    const T* Bp = static_cast<const T*>(p.B.p) + n * p.B.sN + g * p.B.sH;
-    const T* Cp = static_cast<const T*>(p.C.p) + n * p.C.sN + g * p.C.sH;
-    auto fetch_bc = [&](int t) {
 #pragma unroll
         for (int i = 0; i < BC; i++) {
-            const int e = i * kScanWarps * 32 + threadIdx.x, u = t + e / S4, s = e % S4;
-            const bool on = e < TT * S4 && u < t1 && s < p.S;
-            rB[i] = on ? to_f32(Bp[u * p.B.sL + s]) : 0.f;
-            if (PASS == SCAN_WHOLE) rC[i] = on ? to_f32(Cp[u * p.C.sL + s]) : 0.f;
+            const int u = min(t + bc_row + i * (NT / S4), t1 - 1);
+            rB[i] = Bp[u * p.B.sL];
+            if (WHOLE) rC[i] = Cp[u * p.C.sL];
         }
     };
-    if (t0 < t1) { fetch(t0); fetch_bc(t0); }
+    if (t0 < t1) fetch(t0);
     int par = 0;
     for (int t = t0; t < t1; t += TT, par ^= 1) {
         float kx[OS], kz[OS];
 #pragma unroll
         for (int i = 0; i < BC; i++) {
-            const int e = i * kScanWarps * 32 + threadIdx.x;
-            if (e < TT * S4) {
-                sm.B[par][e / S4][e % S4] = rB[i];
-                if (PASS == SCAN_WHOLE) sm.C[par][e / S4][e % S4] = rC[i];
+            const int r = bc_row + i * (NT / S4);
+            if (TT * S4 >= NT || bc_row < TT) {
+                const bool in = bc_on && t + r < t1;
+                sm.B[par][r][bc_s] = in ? to_f32(rB[i]) : 0.f;
+                if (WHOLE) sm.C[par][r][bc_s] = in ? to_f32(rC[i]) : 0.f;
             }
         }
 #pragma unroll
         for (int i = 0; i < OS; i++) {
-            const int u = t + so + i * SP;
-            float d = rd[i] + bias;
-            if (p.softplus) d = softplus_(d);
-            d = mine && u < t1 ? d : 0.f;       // a step behind the end leaves the state as it is
-            sm.delta[warp][so + i * SP][co] = d;
-            sm.dx[warp][so + i * SP][co] = d * rx[i];
-            if (PASS == SCAN_ENDS) dsum += d;
-            kx[i] = rx[i];
-            kz[i] = PASS == SCAN_WHOLE && gated && mine && u < t1 ? to_f32(z[u * p.z.sL]) : 0.f;
+            const bool in = t + j + i * LPC < t1;           // a step behind the end leaves the state as it is
+            kx[i] = to_f32(rx[i]);
+            if (WHOLE && gated) kz[i] = to_f32(rz[i]);
+            float dl = to_f32(rd[i]) + bias;
+            if (p.softplus) dl = softplus_(dl);
+            dl = in ? dl : 0.f;
+            const float dx = in ? dl * kx[i] : 0.f;
+            sm.st[warp][j + i * LPC][grp] = make_float4(dl, dl, dx, dx);
+            if (!WHOLE) dsum += dl;
         }
         __syncthreads();            // B and C of this tile are there; those of the tile before last are free
-        if (t + TT < t1) { fetch(t + TT); fetch_bc(t + TT); }
+        if (t + TT < t1) fetch(t + TT);
 #pragma unroll
         for (int i = 0; i < OS; i++) {
             float v[LPC];
-            if (PASS == SCAN_WHOLE && p.checkpoints && (i * SP) % 8 == 0 && t + i * SP < t1) scan_checkpoint<LPC, CH>(p, n, t + i * SP, g * per, per, cw + CH * grp, j, h);
 #pragma unroll
-            for (int k = 0; k < SP; k++) {
-                const int r = i * SP + k;
-                if (PASS == SCAN_WHOLE && SP > 8 && p.checkpoints && k == 8 && t + r < t1)
-                    scan_checkpoint<LPC, CH>(p, n, t + r, g * per, per, cw + CH * grp, j, h);
+            for (int k = 0; k < LPC; k++) {
+                const int r = i * LPC + k;
+                if (WHOLE && r % kScanKeep == 0 && p.checkpoints && t + r < t1) scan_checkpoint(p, n, t + r, d, on, j, h);
+                const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(&sm.st[warp][r][grp]);
                 const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&sm.B[par][r][4 * j]);
-                ulonglong2 cc = {};
-                if (PASS == SCAN_WHOLE) cc = *reinterpret_cast<const ulonglong2*>(&sm.C[par][r][4 * j]);
-                float dl[CH], dx[CH];
-                load_smem<CH>(&sm.delta[warp][r][CH * grp], dl);
-                load_smem<CH>(&sm.dx[warp][r][CH * grp], dx);
-#pragma unroll
-                for (int c = 0; c < CH; c++) {
-                    const f2 d2 = f2_pack(dl[c], dl[c]), x2 = f2_pack(dx[c], dx[c]);
-                    const f2 e0 = exp2_pair(fmul2(d2, A[c][0])), e1 = exp2_pair(fmul2(d2, A[c][1]));
-                    h[c][0] = ffma2(e0, h[c][0], fmul2(x2, b.x));
-                    h[c][1] = ffma2(e1, h[c][1], fmul2(x2, b.y));
-                    if (RAGGED) keep_states(h[c], 4 * j, p.S);
-                    if (PASS == SCAN_WHOLE) v[k * CH + c] = f2_hsum(ffma2(cc.y, h[c][1], fmul2(cc.x, h[c][0])));
+                const f2 e0 = exp2_pair(fmul2(s.x, A[0])), e1 = exp2_pair(fmul2(s.x, A[1]));
+                h[0] = ffma2(e0, h[0], fmul2(s.y, b.x));
+                h[1] = ffma2(e1, h[1], fmul2(s.y, b.y));
+                if (RAGGED) keep_states(h, 4 * j, p.S);
+                if (WHOLE) {
+                    const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(&sm.C[par][r][4 * j]);
+                    v[k] = f2_hsum(ffma2(c.y, h[1], fmul2(c.x, h[0])));
                 }
             }
-            if (PASS == SCAN_WHOLE) {
+            if (WHOLE) {
                 sum_lanes<LPC, LPC, 1>(v, lane);
-                const int u = t + so + i * SP;
+                const int u = t + j + i * LPC;
                 float y = fmaf(skip, kx[i], v[0]);
                 if (gated) y *= silu_of(kz[i], sigmoidf_(kz[i]));
-                if (mine && u < t1) out[u * p.out.sL] = from_f32<T>(y);
+                if (on && u < t1) out[u * p.out.sL] = from_f32<T>(y);
             }
         }
-        __syncwarp();               // the warp's delta and dx are read
+        __syncwarp();               // the warp's st is read
     }
-    if (PASS == SCAN_WHOLE && mine)
-        for (int u = max(t0, t1) + so; u < tend; u += SP) out[u * p.out.sL] = from_f32<T>(0.f);
+    if (WHOLE && on)
+        for (int u = max(t0, t1) + j; u < tend; u += LPC) out[u * p.out.sL] = from_f32<T>(0.f);
     // what the span leaves
-    const bool last = span == p.spans - 1;
-    if (PASS == SCAN_ENDS || (last && p.state)) {
+    if (on && (!WHOLE || (span == p.spans - 1 && p.state))) {
+        float s[4];
+        f2_unpack(h[0], s[0], s[1]); f2_unpack(h[1], s[2], s[3]);
 #pragma unroll
-        for (int c = 0; c < CH; c++) {
-            const int ch = cw + CH * grp + c;
-            float s[4];
-            f2_unpack(h[c][0], s[0], s[1]); f2_unpack(h[c][1], s[2], s[3]);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int st = 4 * j + i;
-                if (ch >= per || st >= p.S) continue;
-                if (PASS == SCAN_ENDS) p.ends[(spans_at + g * per + ch) * p.S + st] = s[i];
-                else p.state[n * p.state_sN + (g * per + ch) * p.state_sD + st] = s[i];
-            }
+        for (int i = 0; i < 4; i++) {
+            const int st = 4 * j + i;
+            if (st >= p.S) continue;
+            if (!WHOLE) p.ends[spans_at * p.S + st] = s[i];
+            else p.state[n * p.state_sN + d * p.state_sD + st] = s[i];
         }
     }
-    if (PASS == SCAN_ENDS) {
-        // lanes that share a channel hold sums over different steps
+    if (!WHOLE) {
+        // the lanes of a channel hold sums over different steps
 #pragma unroll
-        for (int o = CH; o < LPC; o <<= 1) dsum += __shfl_xor_sync(0xffffffffu, dsum, o);
-        if (mine && so == 0) p.dsums[spans_at + own] = dsum;
+        for (int o = 1; o < LPC; o <<= 1) dsum += __shfl_xor_sync(0xffffffffu, dsum, o);
+        if (on && j == 0) p.dsums[spans_at] = dsum;
     }
 }
 
@@ -290,66 +273,53 @@ __global__ void __launch_bounds__(128) scan_step_kernel(ScanParams p) {
 }
 
 // ------------------------------------------------------------------------------------------------------------ host side
-// Channels per lane, 1 or several (whole): with several the operands B and C are read once for them, with 1 there are that many times as
-// many warps.  Sixteen channels of four states do not fit a lane's registers with their decay rates.
-constexpr int scan_whole(int lpc) { return lpc <= 8 ? lpc : 4; }
 struct ScanPlan {
-    bool whole;
-    int span, spans;        // steps per span, a multiple of the tile
+    int span, spans;        // steps per span, a multiple of every form's tile
 };
 static ScanPlan scan_plan(int N, int L, int D, int S, int G) {
-    const int lpc = scan_lanes(S), per = D / G;
-    const long long sms = sm_count() > 0 ? sm_count() : 148;
-    auto warps = [&](int cw) { return (long long)N * G * ceil_div(per, cw); };
-    ScanPlan q;
-    const int cw = 32 / lpc * scan_whole(lpc);
-    q.whole = lpc == 1 || warps(cw) >= sms * 8;
-    const int tile = 32;        // a multiple of every form's
-    const long long have = warps(q.whole ? cw : 32 / lpc);
-    int spans = 1;
+    const int cta = 32 / scan_lanes(S) * kScanWarps, tile = 32;
+    const long long sms = sm_count() > 0 ? sm_count() : 148, ctas = (long long)N * G * ceil_div(D / G, cta);
     const int forced = tune_get(T_SCAN_CHUNK, 0);
-    // Spans side by side cost the exponentials of a step twice, so they have to bring more than twice the warps.
-    if (forced > 0) spans = (int)ceil_div(L, ceil_div(forced, tile) * tile);
-    else if (have * 3 <= sms * 8) spans = (int)(sms * 16 / have);
-    const int most = (int)ceil_div(L, 2LL * tile);
-    if (!forced && spans > most) spans = most;
+    long long spans = 1;
+    // Spans side by side form the exponentials of a step twice, so they have to bring more than twice the CTAs, of which an SM holds four.
+    if (forced > 0) spans = ceil_div(L, ceil_div(forced, tile) * tile);
+    else if (ctas * 3 <= sms * 4) {
+        spans = sms * 4 / ctas;
+        const long long most = ceil_div(L, 4 * tile);
+        if (spans > most) spans = most;
+    }
     if (spans > 4096) spans = 4096;
-    if (spans < 1) spans = 1;
+    ScanPlan q;
     q.span = (int)(ceil_div(ceil_div(L, spans), tile) * tile);
     q.spans = (int)ceil_div(L, q.span);
     return q;
 }
 
-template <typename T, int LPC, int CH, bool RAGGED>
+template <typename T, int LPC, bool RAGGED>
 static int scan_launch(const ScanParams& p, cudaStream_t st) {
-    constexpr int per_cta = 32 / LPC * CH * kScanWarps;
-    const unsigned gx = (unsigned)(p.G * ceil_div(p.D / p.G, per_cta));
+    const unsigned gx = (unsigned)(p.G * ceil_div(p.D / p.G, 32 / LPC * kScanWarps));
     if (p.spans > 1) {
-        if (int rc = launch_dependent(scan_fwd_kernel<T, LPC, CH, RAGGED, SCAN_ENDS>, p, dim3(gx, p.spans - 1, p.N), kScanWarps * 32, 0, st, nullptr)) return rc;
+        if (int rc = launch_dependent(scan_fwd_kernel<T, LPC, RAGGED, SCAN_ENDS>, p, dim3(gx, p.spans - 1, p.N), kScanWarps * 32, 0, st, nullptr)) return rc;
         if (int rc = launch_scan_join(p, false, st)) return rc;
     }
-    return launch_dependent(scan_fwd_kernel<T, LPC, CH, RAGGED, SCAN_WHOLE>, p, dim3(gx, p.spans, p.N), kScanWarps * 32, 0, st, "scan_fwd_kernel");
+    return launch_dependent(scan_fwd_kernel<T, LPC, RAGGED, SCAN_WHOLE>, p, dim3(gx, p.spans, p.N), kScanWarps * 32, 0, st, "scan_fwd_kernel");
 }
 template <typename T, int LPC>
-static int scan_lanes_launch(const ScanParams& p, bool whole, cudaStream_t st) {
+static int scan_lanes_launch(const ScanParams& p, cudaStream_t st) {
     if (p.L == 1 && !p.checkpoints)
         return launch_dependent(scan_step_kernel<T, LPC>, p, dim3((unsigned)ceil_div((long long)p.D * LPC, 128), (unsigned)ceil_div(p.N, kStepSeqs)),
                                 128, 0, st, "scan_step_kernel");
-    const bool ragged = p.S != 4 * LPC;
-    constexpr int CH = scan_whole(LPC);
-    if (whole) return ragged ? scan_launch<T, LPC, CH, true>(p, st) : scan_launch<T, LPC, CH, false>(p, st);
-    if constexpr (LPC > 1) return ragged ? scan_launch<T, LPC, 1, true>(p, st) : scan_launch<T, LPC, 1, false>(p, st);
-    return FWP_ERR_UNSUPPORTED;
+    return p.S != 4 * LPC ? scan_launch<T, LPC, true>(p, st) : scan_launch<T, LPC, false>(p, st);
 }
 template <typename T>
-static int scan_dispatch(const ScanParams& p, bool whole, cudaStream_t st) {
+static int scan_dispatch(const ScanParams& p, cudaStream_t st) {
     switch (scan_lanes(p.S)) {
-        case 1: return scan_lanes_launch<T, 1>(p, true, st);
-        case 2: return scan_lanes_launch<T, 2>(p, whole, st);
-        case 4: return scan_lanes_launch<T, 4>(p, whole, st);
-        case 8: return scan_lanes_launch<T, 8>(p, whole, st);
+        case 1: return scan_lanes_launch<T, 1>(p, st);
+        case 2: return scan_lanes_launch<T, 2>(p, st);
+        case 4: return scan_lanes_launch<T, 4>(p, st);
+        case 8: return scan_lanes_launch<T, 8>(p, st);
     }
-    return scan_lanes_launch<T, 16>(p, whole, st);
+    return scan_lanes_launch<T, 16>(p, st);
 }
 
 }  // namespace fwp
@@ -402,5 +372,5 @@ FWP_API int fwp_selective_scan_forward(int N, int L, int D, int S, int G, const 
         p.dsums = scratch + (int64_t)N * q.spans * D * S;
     }
     cudaStream_t st = (cudaStream_t)stream;
-    return io_dtype == FWP_F32 ? scan_dispatch<float>(p, q.whole, st) : scan_dispatch<__nv_bfloat16>(p, q.whole, st);
+    return io_dtype == FWP_F32 ? scan_dispatch<float>(p, st) : scan_dispatch<__nv_bfloat16>(p, st);
 }

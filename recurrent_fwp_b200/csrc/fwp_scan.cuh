@@ -102,34 +102,15 @@ __device__ __forceinline__ void keep_states(f2 (&h)[2], int first, int S) {
     h[1] = f2_pack(v[2], v[3]);
 }
 
-template <int CH>
-__device__ __forceinline__ void load_smem(const float* s, float (&v)[CH]) {
-    if constexpr (CH % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < CH; i += 4) {
-            const float4 t = *reinterpret_cast<const float4*>(s + i);
-            v[i] = t.x; v[i + 1] = t.y; v[i + 2] = t.z; v[i + 3] = t.w;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < CH; i++) v[i] = s[i];
-    }
-}
-
-// the state before step t (a multiple of 8) of the lane's channels
-template <int LPC, int CH>
-__device__ __forceinline__ void scan_checkpoint(const ScanParams& p, int n, int t, int base, int per, int ch0, int j, const f2 (&h)[CH][2]) {
+// the state of channel d before step t (a multiple of 8)
+__device__ __forceinline__ void scan_checkpoint(const ScanParams& p, int n, int t, int d, bool on, int j, const f2 (&h)[2]) {
     const int row = scan_row(p.S);
-    float* at = p.checkpoints + (((long long)n * ((p.L + kScanKeep - 1) / kScanKeep) + t / kScanKeep) * p.D + base) * row + 4 * j;
-    if (4 * j >= row) return;
-#pragma unroll
-    for (int c = 0; c < CH; c++)
-        if (ch0 + c < per) {
-            ulonglong2 v;
-            v.x = h[c][0];
-            v.y = h[c][1];
-            *reinterpret_cast<ulonglong2*>(at + (long long)(ch0 + c) * row) = v;
-        }
+    if (!on || 4 * j >= row) return;
+    float* at = p.checkpoints + (((long long)n * ((p.L + kScanKeep - 1) / kScanKeep) + t / kScanKeep) * p.D + d) * row + 4 * j;
+    ulonglong2 v;
+    v.x = h[0];
+    v.y = h[1];
+    *reinterpret_cast<ulonglong2*>(at) = v;
 }
 
 #endif
