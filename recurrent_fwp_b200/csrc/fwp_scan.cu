@@ -4,8 +4,8 @@
 //   y_t = sum_s C_t[s] h_t[s] + skip x_t,  out_t = y_t z_t sigmoid(z_t)
 //
 // Every channel is a recurrence of its own over S states, B and C are shared by the channels of a group.  A lane holds four
-// states of a channel, LPC lanes a channel (S <= 4 LPC).  With LPC steps in hand the sums over s cost LPC - 1 shuffles and leave each lane
-// with the value of one step; that lane loads x, dt, z for it and stores its output, so y goes through no memory.
+// states of two channels, LPC lanes all of them (S <= 4 LPC).  With LPC steps in hand the sums over s cost LPC - 1 shuffles and leave each
+// lane with the value of one step; that lane loads x, dt, z for it and stores its output, so y goes through no memory.
 #include "fwp_scan.cuh"
 
 namespace fwp {
@@ -14,19 +14,19 @@ constexpr int kScanWarps = 4;
 
 template <int LPC>
 struct ScanTile {
-    static constexpr int CW = 32 / LPC;                     // channels per warp
-    static constexpr int OS = LPC == 1 ? 8 : LPC <= 4 ? 4 : 16 / LPC;   // (step, channel) pairs per lane and tile
+    static constexpr int GR = 32 / LPC, CW = 2 * GR;        // lane groups and channels per warp
+    static constexpr int OS = LPC == 1 ? 8 : LPC <= 4 ? 4 : 16 / LPC;   // steps per lane and tile, of two channels each
     static constexpr int TT = OS * LPC;                     // steps per tile
     static constexpr int S4 = 4 * LPC;
-    float4 st[kScanWarps][TT][CW];                          // delta twice, delta x twice: operands of two-wide products as they are
+    float4 st[kScanWarps][TT][kScanGroups<LPC>];                          // delta and delta x of a lane group's two channels
     float B[2][TT][S4];
     float C[2][TT][S4];
 };
 
 // One span of time of one warp's channels.  PASS = SCAN_ENDS: only the state that the span leaves behind, starting from zero, and
 // the sum of delta, for joining spans (scan_join_kernel).
-template <typename T, int LPC, bool RAGGED, int PASS>
-__global__ void __launch_bounds__(kScanWarps * 32, 4) scan_fwd_kernel(ScanParams p) {
+template <typename T, int LPC, bool RAGGED, bool PAIRS, int PASS>
+__global__ void __launch_bounds__(kScanWarps * 32, 3) scan_fwd_kernel(ScanParams p) {
     using Tile = ScanTile<LPC>;
     constexpr int CW = Tile::CW, OS = Tile::OS, TT = Tile::TT, S4 = Tile::S4, NT = kScanWarps * 32;
     constexpr bool WHOLE = PASS == SCAN_WHOLE;
@@ -34,43 +34,47 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) scan_fwd_kernel(ScanParams
     griddep_wait();
     griddep_launch_dependents();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int grp = lane / LPC, j = lane % LPC;             // channel of the warp; its states 4 j ... 4 j + 3, its steps j, j + LPC ...
+    const int grp = lane / LPC, j = lane % LPC;             // two channels; their states 4 j ... 4 j + 3, their steps j, j + LPC ...
     const int n = blockIdx.z, span = blockIdx.y;
     const int per = p.D / p.G, blocks = (per + CW * kScanWarps - 1) / (CW * kScanWarps);
     const int g = blockIdx.x / blocks;
-    const int ch = ((blockIdx.x % blocks) * kScanWarps + warp) * CW + grp;      // inside the group
-    const bool on = ch < per;
-    const int d = g * per + (on ? ch : per - 1);            // a lane without a channel reads the last one's rows and writes nothing
+    const int ch = ((blockIdx.x % blocks) * kScanWarps + warp) * CW + 2 * grp;     // inside the group
+    const bool on[2] = {ch < per, ch + 1 < per};
+    // a lane without a channel reads the last one's rows (the last pair's where they move as pairs: an even channel) and writes nothing
+    const int first = min(ch, per - (PAIRS ? 2 : 1));
+    const int d[2] = {g * per + first, g * per + min(first + 1, per - 1)};
     const int len = p.lengths ? min(max(p.lengths[n], 0), p.L) : p.L;
     const int t0 = span * p.span, tend = min(t0 + p.span, p.L), t1 = min(tend, len);
-    const float bias = p.dt_bias ? p.dt_bias[d] : 0.f, skip = p.skip ? p.skip[d] : 0.f;
     const bool gated = p.z.p != nullptr;
-    const T* x = static_cast<const T*>(p.x.p) + n * p.x.sN + d;
-    const T* dt = static_cast<const T*>(p.dt.p) + n * p.dt.sN + d;
-    const T* z = static_cast<const T*>(p.z.p) + n * p.z.sN + d;
-    T* out = static_cast<T*>(p.out.p) + n * p.out.sN + d;
+    const T* x = static_cast<const T*>(p.x.p) + n * p.x.sN;
+    const T* dt = static_cast<const T*>(p.dt.p) + n * p.dt.sN;
+    const T* z = static_cast<const T*>(p.z.p) + n * p.z.sN;
+    T* out = static_cast<T*>(p.out.p) + n * p.out.sN;
 
-    f2 A[2], h[2];
-    const long long spans_at = ((long long)n * p.spans + span) * p.D + d;       // this span's row in the workspace
-    {
+    f2 A[2][2], h[2][2];
+    float bias[2], skip[2], dsum[2] = {0.f, 0.f};
+    const long long spans_at = ((long long)n * p.spans + span) * p.D;       // this span's rows in the workspace
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+        bias[c] = p.dt_bias ? p.dt_bias[d[c]] : 0.f;
+        skip[c] = p.skip ? p.skip[d[c]] : 0.f;
         float a[4], s[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int st = 4 * j + i;
-            a[i] = st < p.S ? p.A[(long long)d * p.S + st] * kLog2e : 0.f;
+            a[i] = st < p.S ? p.A[(long long)d[c] * p.S + st] * kLog2e : 0.f;
             s[i] = 0.f;
             if (WHOLE && st < p.S) {
-                if (p.spans > 1) s[i] = p.ends[spans_at * p.S + st];
-                else if (p.state) s[i] = p.state[n * p.state_sN + d * p.state_sD + st];
+                if (p.spans > 1) s[i] = p.ends[(spans_at + d[c]) * p.S + st];
+                else if (p.state) s[i] = p.state[n * p.state_sN + d[c] * p.state_sD + st];
             }
         }
-        A[0] = f2_pack(a[0], a[1]); A[1] = f2_pack(a[2], a[3]);
-        h[0] = f2_pack(s[0], s[1]); h[1] = f2_pack(s[2], s[3]);
+        A[c][0] = f2_pack(a[0], a[1]); A[c][1] = f2_pack(a[2], a[3]);
+        h[c][0] = f2_pack(s[0], s[1]); h[c][1] = f2_pack(s[2], s[3]);
     }
-    float dsum = 0.f;
 
     // The next tile's streams, as they are in memory: a conversion here would wait for the load.  Rows behind the end repeat the last one.
-    T rx[OS], rd[OS], rz[OS];
+    Two<T, PAIRS> rx[OS], rd[OS], rz[OS];
     constexpr int BC = (TT * S4 + NT - 1) / NT;
     static_assert((TT * S4) % NT == 0 || TT * S4 < NT, "whole passes over a tile of B and C");
     T rB[BC], rC[BC];
@@ -82,9 +86,9 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) scan_fwd_kernel(ScanParams
 #pragma unroll
         for (int i = 0; i < OS; i++) {
             const int u = min(t + j + i * LPC, t1 - 1);
-            rd[i] = dt[u * p.dt.sL];
-            rx[i] = x[u * p.x.sL];
-            if (WHOLE && gated) rz[i] = z[u * p.z.sL];
+            rd[i].load(dt + u * p.dt.sL, d);
+            rx[i].load(x + u * p.x.sL, d);
+            if (WHOLE && gated) rz[i].load(z + u * p.z.sL, d);
         }
 #pragma unroll
         for (int i = 0; i < BC; i++) {
@@ -96,7 +100,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) scan_fwd_kernel(ScanParams
     if (t0 < t1) fetch(t0);
     int par = 0;
     for (int t = t0; t < t1; t += TT, par ^= 1) {
-        float kx[OS], kz[OS];
+        Two<T, PAIRS> kx[OS], kz[OS];
 #pragma unroll
         for (int i = 0; i < BC; i++) {
             const int r = bc_row + i * (NT / S4);
@@ -109,64 +113,85 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) scan_fwd_kernel(ScanParams
 #pragma unroll
         for (int i = 0; i < OS; i++) {
             const bool in = t + j + i * LPC < t1;           // a step behind the end leaves the state as it is
-            kx[i] = to_f32(rx[i]);
-            if (WHOLE && gated) kz[i] = to_f32(rz[i]);
-            float dl = to_f32(rd[i]) + bias;
-            if (p.softplus) dl = softplus_(dl);
-            dl = in ? dl : 0.f;
-            const float dx = in ? dl * kx[i] : 0.f;
-            sm.st[warp][j + i * LPC][grp] = make_float4(dl, dl, dx, dx);
-            if (!WHOLE) dsum += dl;
+            float dl[2], dx[2];
+            kx[i] = rx[i];
+            if (WHOLE && gated) kz[i] = rz[i];
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                dl[c] = rd[i].get(c) + bias[c];
+                if (p.softplus) dl[c] = softplus_(dl[c]);
+                dl[c] = in ? dl[c] : 0.f;
+                dx[c] = in ? dl[c] * rx[i].get(c) : 0.f;
+                if (!WHOLE) dsum[c] += dl[c];
+            }
+            sm.st[warp][j + i * LPC][grp] = make_float4(dl[0], dx[0], dl[1], dx[1]);
         }
         __syncthreads();            // B and C of this tile are there; those of the tile before last are free
         if (t + TT < t1) fetch(t + TT);
 #pragma unroll
         for (int i = 0; i < OS; i++) {
-            float v[LPC];
+            float v[2][LPC];
 #pragma unroll
             for (int k = 0; k < LPC; k++) {
                 const int r = i * LPC + k;
-                if (WHOLE && r % kScanKeep == 0 && p.checkpoints && t + r < t1) scan_checkpoint(p, n, t + r, d, on, j, h);
-                const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(&sm.st[warp][r][grp]);
+                if (WHOLE && r % kScanKeep == 0 && p.checkpoints && t + r < t1) {
+                    scan_checkpoint(p, n, t + r, d[0], on[0], j, h[0]);
+                    scan_checkpoint(p, n, t + r, d[1], on[1], j, h[1]);
+                }
+                const float4 s = sm.st[warp][r][grp];
                 const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&sm.B[par][r][4 * j]);
-                const f2 e0 = exp2_pair(fmul2(s.x, A[0])), e1 = exp2_pair(fmul2(s.x, A[1]));
-                h[0] = ffma2(e0, h[0], fmul2(s.y, b.x));
-                h[1] = ffma2(e1, h[1], fmul2(s.y, b.y));
-                if (RAGGED) keep_states(h, 4 * j, p.S);
-                if (WHOLE) {
-                    const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(&sm.C[par][r][4 * j]);
-                    v[k] = f2_hsum(ffma2(c.y, h[1], fmul2(c.x, h[0])));
+                ulonglong2 cc = {};
+                if (WHOLE) cc = *reinterpret_cast<const ulonglong2*>(&sm.C[par][r][4 * j]);
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const float dl = c ? s.z : s.x, dx = c ? s.w : s.y;
+                    const f2 d2 = f2_pack(dl, dl), x2 = f2_pack(dx, dx);
+                    const f2 e0 = exp2_pair(fmul2(d2, A[c][0])), e1 = exp2_pair(fmul2(d2, A[c][1]));
+                    h[c][0] = ffma2(e0, h[c][0], fmul2(x2, b.x));
+                    h[c][1] = ffma2(e1, h[c][1], fmul2(x2, b.y));
+                    if (RAGGED) keep_states(h[c], 4 * j, p.S);
+                    if (WHOLE) v[c][k] = f2_hsum(ffma2(cc.y, h[c][1], fmul2(cc.x, h[c][0])));
                 }
             }
             if (WHOLE) {
-                sum_lanes<LPC, LPC, 1>(v, lane);
                 const int u = t + j + i * LPC;
-                float y = fmaf(skip, kx[i], v[0]);
-                if (gated) y *= silu_of(kz[i], sigmoidf_(kz[i]));
-                if (on && u < t1) out[u * p.out.sL] = from_f32<T>(y);
+                float y[2];
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    sum_lanes<LPC, LPC, 1>(v[c], lane);
+                    y[c] = fmaf(skip[c], kx[i].get(c), v[c][0]);
+                    const float zz = gated ? kz[i].get(c) : 0.f;
+                    if (gated) y[c] *= silu_of(zz, sigmoidf_(zz));
+                }
+                if (u < t1) store_two<PAIRS>(out + u * p.out.sL, d, on, y);
             }
         }
         __syncwarp();               // the warp's st is read
     }
-    if (WHOLE && on)
-        for (int u = max(t0, t1) + j; u < tend; u += LPC) out[u * p.out.sL] = from_f32<T>(0.f);
-    // what the span leaves
-    if (on && (!WHOLE || (span == p.spans - 1 && p.state))) {
-        float s[4];
-        f2_unpack(h[0], s[0], s[1]); f2_unpack(h[1], s[2], s[3]);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int st = 4 * j + i;
-            if (st >= p.S) continue;
-            if (!WHOLE) p.ends[spans_at * p.S + st] = s[i];
-            else p.state[n * p.state_sN + d * p.state_sD + st] = s[i];
-        }
+    if (WHOLE) {
+        const float zero[2] = {0.f, 0.f};
+        for (int u = max(t0, t1) + j; u < tend; u += LPC) store_two<PAIRS>(out + u * p.out.sL, d, on, zero);
     }
-    if (!WHOLE) {
-        // the lanes of a channel hold sums over different steps
+    // what the span leaves
 #pragma unroll
-        for (int o = 1; o < LPC; o <<= 1) dsum += __shfl_xor_sync(0xffffffffu, dsum, o);
-        if (on && j == 0) p.dsums[spans_at] = dsum;
+    for (int c = 0; c < 2; c++) {
+        if (on[c] && (!WHOLE || (span == p.spans - 1 && p.state))) {
+            float s[4];
+            f2_unpack(h[c][0], s[0], s[1]); f2_unpack(h[c][1], s[2], s[3]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int st = 4 * j + i;
+                if (st >= p.S) continue;
+                if (!WHOLE) p.ends[(spans_at + d[c]) * p.S + st] = s[i];
+                else p.state[n * p.state_sN + d[c] * p.state_sD + st] = s[i];
+            }
+        }
+        if (!WHOLE) {
+            // the lanes of a channel hold sums over different steps
+#pragma unroll
+            for (int o = 1; o < LPC; o <<= 1) dsum[c] += __shfl_xor_sync(0xffffffffu, dsum[c], o);
+            if (on[c] && j == 0) p.dsums[spans_at + d[c]] = dsum[c];
+        }
     }
 }
 
@@ -277,14 +302,14 @@ struct ScanPlan {
     int span, spans;        // steps per span, a multiple of every form's tile
 };
 static ScanPlan scan_plan(int N, int L, int D, int S, int G) {
-    const int cta = 32 / scan_lanes(S) * kScanWarps, tile = 32;
+    const int cta = 64 / scan_lanes(S) * kScanWarps, tile = 32;
     const long long sms = sm_count() > 0 ? sm_count() : 148, ctas = (long long)N * G * ceil_div(D / G, cta);
     const int forced = tune_get(T_SCAN_CHUNK, 0);
     long long spans = 1;
-    // Spans side by side form the exponentials of a step twice, so they have to bring more than twice the CTAs, of which an SM holds four.
+    // Spans side by side form the exponentials of a step twice, so they have to bring more than twice the CTAs, of which an SM holds two to three.
     if (forced > 0) spans = ceil_div(L, ceil_div(forced, tile) * tile);
-    else if (ctas * 3 <= sms * 4) {
-        spans = sms * 4 / ctas;
+    else if (ctas * 3 <= sms * 2) {
+        spans = sms * 2 / ctas;
         const long long most = ceil_div(L, 4 * tile);
         if (spans > most) spans = most;
     }
@@ -295,21 +320,22 @@ static ScanPlan scan_plan(int N, int L, int D, int S, int G) {
     return q;
 }
 
-template <typename T, int LPC, bool RAGGED>
+template <typename T, int LPC, bool RAGGED, bool PAIRS>
 static int scan_launch(const ScanParams& p, cudaStream_t st) {
-    const unsigned gx = (unsigned)(p.G * ceil_div(p.D / p.G, 32 / LPC * kScanWarps));
+    const unsigned gx = (unsigned)(p.G * ceil_div(p.D / p.G, 64 / LPC * kScanWarps));
     if (p.spans > 1) {
-        if (int rc = launch_dependent(scan_fwd_kernel<T, LPC, RAGGED, SCAN_ENDS>, p, dim3(gx, p.spans - 1, p.N), kScanWarps * 32, 0, st, nullptr)) return rc;
+        if (int rc = launch_dependent(scan_fwd_kernel<T, LPC, RAGGED, PAIRS, SCAN_ENDS>, p, dim3(gx, p.spans - 1, p.N), kScanWarps * 32, 0, st, nullptr)) return rc;
         if (int rc = launch_scan_join(p, false, st)) return rc;
     }
-    return launch_dependent(scan_fwd_kernel<T, LPC, RAGGED, SCAN_WHOLE>, p, dim3(gx, p.spans, p.N), kScanWarps * 32, 0, st, "scan_fwd_kernel");
+    return launch_dependent(scan_fwd_kernel<T, LPC, RAGGED, PAIRS, SCAN_WHOLE>, p, dim3(gx, p.spans, p.N), kScanWarps * 32, 0, st, "scan_fwd_kernel");
 }
 template <typename T, int LPC>
 static int scan_lanes_launch(const ScanParams& p, cudaStream_t st) {
     if (p.L == 1 && !p.checkpoints)
         return launch_dependent(scan_step_kernel<T, LPC>, p, dim3((unsigned)ceil_div((long long)p.D * LPC, 128), (unsigned)ceil_div(p.N, kStepSeqs)),
                                 128, 0, st, "scan_step_kernel");
-    return p.S != 4 * LPC ? scan_launch<T, LPC, true>(p, st) : scan_launch<T, LPC, false>(p, st);
+    if (p.S != 4 * LPC) return scan_launch<T, LPC, true, false>(p, st);
+    return p.pairs ? scan_launch<T, LPC, false, true>(p, st) : scan_launch<T, LPC, false, false>(p, st);
 }
 template <typename T>
 static int scan_dispatch(const ScanParams& p, cudaStream_t st) {
@@ -362,6 +388,8 @@ FWP_API int fwp_selective_scan_forward(int N, int L, int D, int S, int G, const 
         p.state_vec = S % 4 == 0 && aligned16(p.state) && p.state_sN % 4 == 0 && p.state_sD % 4 == 0;
     }
     p.checkpoints = checkpoints;
+    p.pairs = D / G % 2 == 0 && rows_aligned(p.x, esz, 2 * esz) && rows_aligned(p.dt, esz, 2 * esz) && rows_aligned(p.z, esz, 2 * esz) &&
+              rows_aligned(p.out, esz, 2 * esz);
     const ScanPlan q = scan_plan(N, L, D, S, G);
     p.span = q.span;
     p.spans = q.spans;

@@ -18,6 +18,7 @@ struct ScanParams {
     float* state;           // (N, D, S), null: zeros
     long long state_sN, state_sD;
     bool state_vec;         // rows of the state move in 16-byte pieces
+    bool pairs;             // the rows of two neighbouring channels move as one
     float* checkpoints;     // [N][ceil(L / 8)][D][scan_row(S)]
     float *ends, *dsums;    // [N][spans][D][S] and [N][spans][D]
     int N, L, D, S, G, softplus, span, spans;
@@ -100,6 +101,46 @@ __device__ __forceinline__ void keep_states(f2 (&h)[2], int first, int S) {
     for (int i = 0; i < 4; i++) v[i] = first + i < S ? v[i] : 0.f;
     h[0] = f2_pack(v[0], v[1]);
     h[1] = f2_pack(v[2], v[3]);
+}
+
+// One row's values of two channels as they are in memory, one word where they are neighbours that move as one (PAIRS).  They are taken
+// apart and converted where they are used: an instruction next to the load would wait for it.
+// entries of 16 bytes per lane group between a step's row and the next, so that the eight lanes that store at once meet no bank twice
+template <int LPC> constexpr int kScanGroups = 32 / LPC + (LPC == 1 ? 0 : LPC == 2 ? 4 : LPC == 4 ? 2 : 1);
+
+template <typename T, bool PAIRS> struct Two;
+template <typename T> struct Two<T, false> {
+    T v[2];
+    __device__ __forceinline__ void load(const T* row, const int (&d)[2]) { v[0] = row[d[0]]; v[1] = row[d[1]]; }
+    __device__ __forceinline__ float get(int c) const { return to_f32(v[c]); }
+};
+template <> struct Two<float, true> {
+    float2 v;
+    __device__ __forceinline__ void load(const float* row, const int (&d)[2]) { v = *reinterpret_cast<const float2*>(row + d[0]); }
+    __device__ __forceinline__ float get(int c) const { return c ? v.y : v.x; }
+};
+template <> struct Two<__nv_bfloat16, true> {
+    unsigned v;
+    __device__ __forceinline__ void load(const __nv_bfloat16* row, const int (&d)[2]) { v = *reinterpret_cast<const unsigned*>(row + d[0]); }
+    __device__ __forceinline__ float get(int c) const { return __uint_as_float(c ? v & 0xffff0000u : v << 16); }
+};
+template <bool PAIRS>
+__device__ __forceinline__ void store_two(float* row, const int (&d)[2], const bool (&on)[2], const float (&v)[2]) {
+    if (PAIRS) {
+        if (on[0]) *reinterpret_cast<float2*>(row + d[0]) = make_float2(v[0], v[1]);
+    } else {
+        if (on[0]) row[d[0]] = v[0];
+        if (on[1]) row[d[1]] = v[1];
+    }
+}
+template <bool PAIRS>
+__device__ __forceinline__ void store_two(__nv_bfloat16* row, const int (&d)[2], const bool (&on)[2], const float (&v)[2]) {
+    if (PAIRS) {
+        if (on[0]) *reinterpret_cast<__nv_bfloat162*>(row + d[0]) = __floats2bfloat162_rn(v[0], v[1]);
+    } else {
+        if (on[0]) row[d[0]] = from_f32<__nv_bfloat16>(v[0]);
+        if (on[1]) row[d[1]] = from_f32<__nv_bfloat16>(v[1]);
+    }
 }
 
 // the state of channel d before step t (a multiple of 8)
