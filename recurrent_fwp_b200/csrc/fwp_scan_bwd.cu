@@ -60,9 +60,9 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 2) scan_bwd_kernel(ScanParams 
     const int n = blockIdx.z, span = WHOLE ? blockIdx.y : blockIdx.y + 1;       // nothing in front of the first span asks for its end
     const int per = p.D / p.G, blocks = (per + CW * kBwdWarps - 1) / (CW * kBwdWarps);
     const int g = blockIdx.x / blocks;
-    const int wch = ((blockIdx.x % blocks) * kBwdWarps + warp) * CW, ch = wch + 2 * grp;     // inside the group
-    const bool on[2] = {ch < per, ch + 1 < per}, full = wch + CW <= per;        // full: every lane of the warp has its channels
-    const int last = min(ch, per - (PAIRS ? 2 : 1));        // a lane without a channel reads the last one's rows and writes nothing
+    const int ch = ((blockIdx.x % blocks) * kBwdWarps + warp) * CW + 2 * grp;                // inside the group
+    const bool on[2] = {ch < per, ch + 1 < per};
+    const int last = min(ch, per - (PAIRS ? 2 : 1));        // a lane without a channel reads the last one's rows, counts as steps behind the end, and writes nothing
     const int d[2] = {g * per + last, g * per + min(last + 1, per - 1)};
     const int len = p.lengths ? min(max(p.lengths[n], 0), p.L) : p.L;
     const int t0 = span * p.span, tend = min(t0 + p.span, p.L), t1 = min(tend, len);
@@ -174,11 +174,11 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 2) scan_bwd_kernel(ScanParams 
 #pragma unroll
             for (int i = 0; i < OS; i++) {
                 const int r = kHalf * hh + os + i;
-                const bool in = t + r < t1;
                 float dl[NC], dx[NC], gy[NC];
                 if (WHOLE) kx[hh][i] = rx[hh][i];
 #pragma unroll
                 for (int c = 0; c < NC; c++) {
+                    const bool in = t + r < t1 && on[NC == 2 ? c : oc];
                     const float raw = rd[hh][i].get(c) + bias[c];
                     dl[c] = raw;
                     sig[hh][i][c] = 1.f;
@@ -301,12 +301,8 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 2) scan_bwd_kernel(ScanParams 
                     q[2 * r + c] = f2_hsum(ffma2(e1, A[c][1], fmul2(e0, A[c][0])));
                     part[c][0] = ffma2(e0, d2, part[c][0]);
                     part[c][1] = ffma2(e1, d2, part[c][1]);
-                    // a lane without a channel adds nothing, whatever the last one's rows hold
-                    const bool adds = full || on[c];
-                    const f2 pb0 = adds ? fmul2(gg[0], x2) : 0, pb1 = adds ? fmul2(gg[1], x2) : 0;
-                    const f2 pc0 = adds ? fmul2(gy2, H[r][c][0]) : 0, pc1 = adds ? fmul2(gy2, H[r][c][1]) : 0;
-                    gB0 = c ? fadd2(gB0, pb0) : pb0; gB1 = c ? fadd2(gB1, pb1) : pb1;
-                    gC0 = c ? fadd2(gC0, pc0) : pc0; gC1 = c ? fadd2(gC1, pc1) : pc1;
+                    gB0 = c ? ffma2(gg[0], x2, gB0) : fmul2(gg[0], x2); gB1 = c ? ffma2(gg[1], x2, gB1) : fmul2(gg[1], x2);
+                    gC0 = c ? ffma2(gy2, H[r][c][0], gC0) : fmul2(gy2, H[r][c][0]); gC1 = c ? ffma2(gy2, H[r][c][1], gC1) : fmul2(gy2, H[r][c][1]);
                 }
                 float w[8];
                 f2_unpack(gB0, w[0], w[1]);
