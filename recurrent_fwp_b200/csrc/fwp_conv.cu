@@ -7,13 +7,14 @@
 // of one sequence and walks a span of steps with the last K - 1 inputs in registers, so every input is read once (and K - 1 of
 // a neighbour's span, from L2); eight rows are in flight per warp.  The backward walks forwards too: it forms p again from
 // the inputs it needs for gw anyway, and gx K - 1 steps behind.
+#include <type_traits>
 #include "fwp_seq.cuh"
 
 namespace fwp {
 
 constexpr int kConvMaxK = 8;
 constexpr int kConvWarps = 4;
-constexpr int kConvRows = 8;            // rows loaded ahead of their use
+constexpr int kConvSpan = 8;            // the shortest span: above K - 1, so that the first span alone sees the state
 
 struct ConvParams {
     Stream x, state, out, gout, gx;     // state: rows are the K - 1 inputs before the first
@@ -49,6 +50,7 @@ __device__ __forceinline__ void conv_window(const ConvParams& p, const T* x, int
 
 template <typename T, int K, int V>
 __global__ void __launch_bounds__(kConvWarps * 32) conv_fwd_kernel(ConvParams p) {
+    constexpr int ROWS = V == 4 ? 4 : 8;           // rows loaded ahead of their use
     griddep_wait();
     griddep_launch_dependents();
     const int lane = threadIdx.x & 31, n = blockIdx.z;
@@ -70,45 +72,41 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_fwd_kernel(ConvParams p)
         float end[K][V];
 #pragma unroll
         for (int j = 0; j < K - 1; j++) {
-            const int t = len - (K - 1) + j;
-#pragma unroll
-            for (int i = 0; i < V; i++) end[j][i] = 0.f;
-            if (t >= 0) load_vec<V>(x + t * p.x.sL, end[j]);
-            else {
-                // input t lies in the old state, at row t + K - 1
-#pragma unroll
-                for (int q = 0; q < K - 1; q++)
-                    if (q == t + K - 1) {
-#pragma unroll
-                        for (int i = 0; i < V; i++) end[j][i] = win[q][i];
-                    }
-            }
+            // the inputs and the state before them are one sequence: K - 1 rows of state, then x; its rows from len on
+            if (len + j >= K - 1) load_vec<V>(x + (len + j - (K - 1)) * p.x.sL, end[j]);
+            else load_vec<V>(st + (len + j) * p.state.sL, end[j]);
         }
 #pragma unroll
         for (int j = 0; j < K - 1; j++) store_vec<V>(st + j * p.state.sL, end[j]);
     }
-    for (int t = t0; t < t1; t += kConvRows) {
-        float in[kConvRows][V];
+    if (t0 < t1) {
+        RawVec<T, V> raw[ROWS];        // rows behind the end repeat the last one
+        auto fetch = [&](int t) {
 #pragma unroll
-        for (int r = 0; r < kConvRows; r++) {
+            for (int r = 0; r < ROWS; r++) raw[r].load(x + min(t + r, t1 - 1) * p.x.sL);
+        };
+        fetch(t0);
+        for (int t = t0; t < t1; t += ROWS) {
+            RawVec<T, V> now[ROWS];
 #pragma unroll
-            for (int i = 0; i < V; i++) in[r][i] = 0.f;
-            if (t + r < t1) load_vec<V>(x + (long long)(t + r) * p.x.sL, in[r]);
-        }
+            for (int r = 0; r < ROWS; r++) now[r] = raw[r];
+            if (t + ROWS < t1) fetch(t + ROWS);
+            T* to = out + t * p.out.sL;
 #pragma unroll
-        for (int r = 0; r < kConvRows; r++) {
-            float y[V];
+            for (int r = 0; r < ROWS; r++) {
+                float y[V];
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                win[K - 1][i] = in[r][i];
-                float a = b[i];
+                for (int i = 0; i < V; i++) {
+                    win[K - 1][i] = now[r].get(i);
+                    float a = b[i];
 #pragma unroll
-                for (int j = 0; j < K; j++) a = fmaf(w[j][i], win[j][i], a);
-                y[i] = p.silu ? a * sigmoidf_(a) : a;
+                    for (int j = 0; j < K; j++) a = fmaf(w[j][i], win[j][i], a);
+                    y[i] = p.silu ? a * sigmoidf_(a) : a;
 #pragma unroll
-                for (int j = 0; j < K - 1; j++) win[j][i] = win[j + 1][i];
+                    for (int j = 0; j < K - 1; j++) win[j][i] = win[j + 1][i];
+                }
+                if (t + r < t1) store_vec<V>(to + r * p.out.sL, y);
             }
-            if (t + r < t1) store_vec<V>(out + (long long)(t + r) * p.out.sL, y);
         }
     }
     const float zero[V] = {};
@@ -118,6 +116,7 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_fwd_kernel(ConvParams p)
 template <typename T, int K, int V>
 __global__ void __launch_bounds__(kConvWarps * 32) conv_bwd_kernel(ConvParams p) {
     __shared__ float red[kConvWarps][K + 1][32 * V];
+    constexpr int ROWS = 4;
     griddep_wait();
     griddep_launch_dependents();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockIdx.z;
@@ -145,33 +144,38 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_bwd_kernel(ConvParams p)
             for (int j = 0; j < K; j++)
 #pragma unroll
                 for (int i = 0; i < V; i++) gp[j][i] = 0.f;
-            const int uend = t1 + K - 1;                   // steps from t1 on belong to the next span: only their gp counts here
-            for (int u0 = t0; u0 < uend; u0 += kConvRows) {
-                float in[kConvRows][V], go[kConvRows][V];
+            const int uend = min(t1 + K - 1, len), ulast = uend - 1;     // steps from t1 on belong to the next span: only their gp counts here
+            RawVec<T, V> rx[ROWS], rg[ROWS];
+            auto fetch = [&](int u) {
 #pragma unroll
-                for (int r = 0; r < kConvRows; r++) {
-#pragma unroll
-                    for (int i = 0; i < V; i++) in[r][i] = go[r][i] = 0.f;
-                    if (u0 + r < min(uend, len)) {
-                        load_vec<V>(x + (long long)(u0 + r) * p.x.sL, in[r]);
-                        load_vec<V>(gout + (long long)(u0 + r) * p.gout.sL, go[r]);
-                    }
+                for (int r = 0; r < ROWS; r++) {
+                    rx[r].load(x + min(u + r, ulast) * p.x.sL);
+                    rg[r].load(gout + min(u + r, ulast) * p.gout.sL);
                 }
+            };
+            // eight steps from u0 on; INNER: all of them count in full, and so do the steps K - 1 before them
+            auto block = [&](auto inner, int u0) {
+                constexpr bool INNER = decltype(inner)::value;
+                RawVec<T, V> nx[ROWS], ng[ROWS];
 #pragma unroll
-                for (int r = 0; r < kConvRows; r++) {
+                for (int r = 0; r < ROWS; r++) { nx[r] = rx[r]; ng[r] = rg[r]; }
+                if (u0 + ROWS < uend) fetch(u0 + ROWS);
+                T* to = gx + (u0 - (K - 1)) * p.gx.sL;
+#pragma unroll
+                for (int r = 0; r < ROWS; r++) {
                     const int u = u0 + r;
                     float g[V];
 #pragma unroll
                     for (int i = 0; i < V; i++) {
-                        win[K - 1][i] = in[r][i];
+                        win[K - 1][i] = nx[r].get(i);
                         float a = b[i];
 #pragma unroll
                         for (int j = 0; j < K; j++) a = fmaf(w[j][i], win[j][i], a);
-                        float d = go[r][i];
+                        float d = ng[r].get(i);
                         if (p.silu) d *= silu_grad_of(a, sigmoidf_(a));
-                        d = u < len ? d : 0.f;
+                        if (!INNER) d = u < uend ? d : 0.f;
                         gp[K - 1][i] = d;
-                        if (u < t1) {
+                        if (INNER || u < t1) {
                             gb[i] += d;
 #pragma unroll
                             for (int j = 0; j < K; j++) gw[j][i] = fmaf(d, win[j][i], gw[j][i]);
@@ -184,8 +188,13 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_bwd_kernel(ConvParams p)
                         for (int j = 0; j < K - 1; j++) { win[j][i] = win[j + 1][i]; gp[j][i] = gp[j + 1][i]; }
                     }
                     const int t = u - (K - 1);
-                    if (t >= t0 && t < t1) store_vec<V>(gx + (long long)t * p.gx.sL, g);
+                    if (INNER || (t >= t0 && t < t1)) store_vec<V>(to + r * p.gx.sL, g);
                 }
+            };
+            fetch(t0);
+            for (int u0 = t0; u0 < t1 + K - 1; u0 += ROWS) {
+                if (u0 - (K - 1) >= t0 && u0 + ROWS <= t1) block(std::true_type(), u0);
+                else block(std::false_type(), u0);
             }
         }
         const float zero[V] = {};
@@ -214,7 +223,7 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_bwd_kernel(ConvParams p)
 static int conv_span(int N, int L, int D, int V) {
     const long long columns = (long long)N * ceil_div(D, 32 * V), sms = sm_count() > 0 ? sm_count() : 148;
     int span = 64;
-    while (span > kConvRows && columns * ceil_div(L, span) < sms * 16) span >>= 1;
+    while (span > kConvSpan && columns * ceil_div(L, span) < sms * 16) span >>= 1;
     while (ceil_div(L, (long long)span * kConvWarps) > 65535) span <<= 1;      // the grid's limit
     return span;
 }

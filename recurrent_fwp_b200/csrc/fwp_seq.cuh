@@ -83,6 +83,27 @@ __device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float (&v)[V])
     }
 }
 
+// V elements as they are in memory, converted where they are used: a conversion next to the load would wait for it
+template <typename T, int V> struct RawVec;
+template <typename T> struct RawVec<T, 1> {
+    T v;
+    __device__ __forceinline__ void load(const T* p) { v = *p; }
+    __device__ __forceinline__ float get(int) const { return to_f32(v); }
+};
+template <> struct RawVec<float, 4> {
+    float4 v;
+    __device__ __forceinline__ void load(const float* p) { v = *reinterpret_cast<const float4*>(p); }
+    __device__ __forceinline__ float get(int i) const { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+};
+template <> struct RawVec<__nv_bfloat16, 4> {
+    uint2 v;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = *reinterpret_cast<const uint2*>(p); }
+    __device__ __forceinline__ float get(int i) const {
+        const unsigned w = i < 2 ? v.x : v.y;
+        return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+    }
+};
+
 // Sums of `n` values over LANES lanes that are STRIDE apart.  While there are more values than one the halves of the lanes take half of
 // the values each (n / 2 shuffles), afterwards plain butterflies.  Where n >= LANES a lane ends with n / LANES values: those whose index
 // is i * LANES... in the order of bits: the lane with index l = (lane / STRIDE) % LANES holds values l * (n / LANES) ... + n / LANES - 1
