@@ -24,33 +24,81 @@ struct ConvParams {
     int N, L, D, silu, span, spans, groups;     // groups: of 32 x V channels
 };
 
+// V neighbouring channels of a step: one float, or two pairs for the two-wide instructions
+template <int V> struct Lanes;
+template <> struct Lanes<1> {
+    float v;
+    __device__ __forceinline__ static Lanes all(float x) { return {x}; }
+    __device__ __forceinline__ static Lanes of(const float (&x)[1]) { return {x[0]}; }
+    __device__ __forceinline__ void get(float (&x)[1]) const { x[0] = v; }
+};
+template <> struct Lanes<4> {
+    f2 v[2];
+    __device__ __forceinline__ static Lanes all(float x) { return {{f2_pack(x, x), f2_pack(x, x)}}; }
+    __device__ __forceinline__ static Lanes of(const float (&x)[4]) { return {{f2_pack(x[0], x[1]), f2_pack(x[2], x[3])}}; }
+    __device__ __forceinline__ void get(float (&x)[4]) const { f2_unpack(v[0], x[0], x[1]); f2_unpack(v[1], x[2], x[3]); }
+};
+__device__ __forceinline__ Lanes<1> fma_(Lanes<1> a, Lanes<1> b, Lanes<1> c) { return {fmaf(a.v, b.v, c.v)}; }
+__device__ __forceinline__ Lanes<1> mul_(Lanes<1> a, Lanes<1> b) { return {a.v * b.v}; }
+__device__ __forceinline__ Lanes<1> add_(Lanes<1> a, Lanes<1> b) { return {a.v + b.v}; }
+__device__ __forceinline__ Lanes<4> fma_(Lanes<4> a, Lanes<4> b, Lanes<4> c) { return {{ffma2(a.v[0], b.v[0], c.v[0]), ffma2(a.v[1], b.v[1], c.v[1])}}; }
+__device__ __forceinline__ Lanes<4> mul_(Lanes<4> a, Lanes<4> b) { return {{fmul2(a.v[0], b.v[0]), fmul2(a.v[1], b.v[1])}}; }
+__device__ __forceinline__ Lanes<4> add_(Lanes<4> a, Lanes<4> b) { return {{fadd2(a.v[0], b.v[0]), fadd2(a.v[1], b.v[1])}}; }
+template <int V>
+__device__ __forceinline__ Lanes<V> sigmoid_(Lanes<V> a) {
+    float e[V];
+    mul_(a, Lanes<V>::all(-kLog2e)).get(e);
+#pragma unroll
+    for (int i = 0; i < V; i++) e[i] = ex2_approx(e[i]);
+    add_(Lanes<V>::of(e), Lanes<V>::all(1.f)).get(e);
+#pragma unroll
+    for (int i = 0; i < V; i++) e[i] = rcp_approx(e[i]);
+    return Lanes<V>::of(e);
+}
+template <typename T, int V>
+__device__ __forceinline__ Lanes<V> lanes_of(const RawVec<T, V>& r) {
+    float x[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) x[i] = r.get(i);
+    return Lanes<V>::of(x);
+}
+template <int V, typename T>
+__device__ __forceinline__ Lanes<V> load_lanes(const T* p) {
+    float x[V];
+    load_vec<V>(p, x);
+    return Lanes<V>::of(x);
+}
+
 template <int K, int V>
-__device__ __forceinline__ void conv_weights(const ConvParams& p, int d0, int nd, float (&w)[K][V], float (&b)[V]) {
+__device__ __forceinline__ void conv_weights(const ConvParams& p, int d0, Lanes<V> (&w)[K], Lanes<V>& b) {
+    float x[V];
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        b[i] = i < nd && p.b ? p.b[d0 + i] : 0.f;
+    for (int i = 0; i < V; i++) x[i] = p.b ? p.b[d0 + i] : 0.f;
+    b = Lanes<V>::of(x);
 #pragma unroll
-        for (int j = 0; j < K; j++) w[j][i] = i < nd ? p.w[(long long)(d0 + i) * K + j] : 0.f;
+    for (int j = 0; j < K; j++) {
+#pragma unroll
+        for (int i = 0; i < V; i++) x[i] = p.w[(long long)(d0 + i) * K + j];
+        w[j] = Lanes<V>::of(x);
     }
 }
 
 // the K - 1 inputs before step t0 (steps below zero come from the state, or are zero)
 template <typename T, int K, int V>
-__device__ __forceinline__ void conv_window(const ConvParams& p, const T* x, int n, int t0, int d0, float (&win)[K][V]) {
+__device__ __forceinline__ void conv_window(const ConvParams& p, const T* x, int n, int t0, int d0, Lanes<V> (&win)[K]) {
 #pragma unroll
     for (int j = 0; j < K - 1; j++) {
         const int t = t0 - (K - 1) + j;
-#pragma unroll
-        for (int i = 0; i < V; i++) win[j][i] = 0.f;
-        if (t >= 0) load_vec<V>(x + t * p.x.sL, win[j]);
+        win[j] = Lanes<V>::all(0.f);
+        if (t >= 0) win[j] = load_lanes<V>(x + t * p.x.sL);
         else if (p.state.p)
-            load_vec<V>(static_cast<const float*>(p.state.p) + n * p.state.sN + (long long)(t + K - 1) * p.state.sL + d0, win[j]);
+            win[j] = load_lanes<V>(static_cast<const float*>(p.state.p) + n * p.state.sN + (long long)(t + K - 1) * p.state.sL + d0);
     }
 }
 
 template <typename T, int K, int V>
-__global__ void __launch_bounds__(kConvWarps * 32) conv_fwd_kernel(ConvParams p) {
-    constexpr int ROWS = V == 4 ? 4 : 8;           // rows loaded ahead of their use
+__global__ void __launch_bounds__(kConvWarps * 32, K <= 4 ? 5 : 3) conv_fwd_kernel(ConvParams p) {
+    constexpr int ROWS = V == 4 && sizeof(T) == 4 ? 4 : 8;           // rows loaded ahead of their use
     griddep_wait();
     griddep_launch_dependents();
     const int lane = threadIdx.x & 31, n = blockIdx.z;
@@ -61,9 +109,9 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_fwd_kernel(ConvParams p)
     const int t0 = s * p.span, t1 = min(t0 + p.span, len), tend = min(t0 + p.span, p.L);
     const T* x = static_cast<const T*>(p.x.p) + n * p.x.sN + d0;
     T* out = static_cast<T*>(p.out.p) + n * p.out.sN + d0;
-    float w[K][V], b[V], win[K][V];
+    Lanes<V> w[K], b, win[K];
     if (t0 < t1 || s == 0) {
-        conv_weights<K, V>(p, d0, V, w, b);
+        conv_weights<K, V>(p, d0, w, b);
         conv_window<T, K, V>(p, x, n, t0, d0, win);
     }
     // the first span reads the state before the steps, and writes the one behind them: nobody else touches it
@@ -94,17 +142,15 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_fwd_kernel(ConvParams p)
             T* to = out + t * p.out.sL;
 #pragma unroll
             for (int r = 0; r < ROWS; r++) {
+                win[K - 1] = lanes_of(now[r]);
+                Lanes<V> a = b;
+#pragma unroll
+                for (int j = 0; j < K; j++) a = fma_(w[j], win[j], a);
+                if (p.silu) a = mul_(a, sigmoid_(a));
+#pragma unroll
+                for (int j = 0; j < K - 1; j++) win[j] = win[j + 1];
                 float y[V];
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-                    win[K - 1][i] = now[r].get(i);
-                    float a = b[i];
-#pragma unroll
-                    for (int j = 0; j < K; j++) a = fmaf(w[j][i], win[j][i], a);
-                    y[i] = p.silu ? a * sigmoidf_(a) : a;
-#pragma unroll
-                    for (int j = 0; j < K - 1; j++) win[j][i] = win[j + 1][i];
-                }
+                a.get(y);
                 if (t + r < t1) store_vec<V>(to + r * p.out.sL, y);
             }
         }
@@ -114,22 +160,19 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_fwd_kernel(ConvParams p)
 }
 
 template <typename T, int K, int V>
-__global__ void __launch_bounds__(kConvWarps * 32) conv_bwd_kernel(ConvParams p) {
-    __shared__ float red[kConvWarps][K + 1][32 * V];
+__global__ void __launch_bounds__(kConvWarps * 32, K > 4 ? 2 : sizeof(T) == 2 ? 4 : 3) conv_bwd_kernel(ConvParams p) {
     constexpr int ROWS = 4;
+    __shared__ float red[kConvWarps][K + 1][32 * V];
     griddep_wait();
     griddep_launch_dependents();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockIdx.z;
     const int d0 = (blockIdx.x * 32 + lane) * V;
     const int s = blockIdx.y * kConvWarps + warp;
     const bool on = d0 < p.D && s < p.spans;
-    float gw[K][V], gb[V];
+    const Lanes<V> none = Lanes<V>::all(0.f), one = Lanes<V>::all(1.f);
+    Lanes<V> gw[K], gb = none;
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        gb[i] = 0.f;
-#pragma unroll
-        for (int j = 0; j < K; j++) gw[j][i] = 0.f;
-    }
+    for (int j = 0; j < K; j++) gw[j] = none;
     if (on) {
         const int len = p.lengths ? min(max(p.lengths[n], 0), p.L) : p.L;
         const int t0 = s * p.span, t1 = min(t0 + p.span, len), tend = min(t0 + p.span, p.L);
@@ -137,13 +180,11 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_bwd_kernel(ConvParams p)
         const T* gout = static_cast<const T*>(p.gout.p) + n * p.gout.sN + d0;
         T* gx = static_cast<T*>(p.gx.p) + n * p.gx.sN + d0;
         if (t0 < t1) {
-            float w[K][V], b[V], win[K][V], gp[K][V];      // gp[j]: of step u - K + 1 + j
-            conv_weights<K, V>(p, d0, V, w, b);
+            Lanes<V> w[K], b, win[K], gp[K];               // gp[j]: of step u - K + 1 + j
+            conv_weights<K, V>(p, d0, w, b);
             conv_window<T, K, V>(p, x, n, t0, d0, win);
 #pragma unroll
-            for (int j = 0; j < K; j++)
-#pragma unroll
-                for (int i = 0; i < V; i++) gp[j][i] = 0.f;
+            for (int j = 0; j < K; j++) gp[j] = none;
             const int uend = min(t1 + K - 1, len), ulast = uend - 1;     // steps from t1 on belong to the next span: only their gp counts here
             RawVec<T, V> rx[ROWS], rg[ROWS];
             auto fetch = [&](int u) {
@@ -153,7 +194,7 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_bwd_kernel(ConvParams p)
                     rg[r].load(gout + min(u + r, ulast) * p.gout.sL);
                 }
             };
-            // eight steps from u0 on; INNER: all of them count in full, and so do the steps K - 1 before them
+            // ROWS steps from u0 on; INNER: all of them count in full, and so do the steps K - 1 before them
             auto block = [&](auto inner, int u0) {
                 constexpr bool INNER = decltype(inner)::value;
                 RawVec<T, V> nx[ROWS], ng[ROWS];
@@ -163,31 +204,30 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_bwd_kernel(ConvParams p)
                 T* to = gx + (u0 - (K - 1)) * p.gx.sL;
 #pragma unroll
                 for (int r = 0; r < ROWS; r++) {
-                    const int u = u0 + r;
-                    float g[V];
+                    const int u = u0 + r, t = u - (K - 1);
+                    win[K - 1] = lanes_of(nx[r]);
+                    Lanes<V> a = b, d = lanes_of(ng[r]);
 #pragma unroll
-                    for (int i = 0; i < V; i++) {
-                        win[K - 1][i] = nx[r].get(i);
-                        float a = b[i];
-#pragma unroll
-                        for (int j = 0; j < K; j++) a = fmaf(w[j][i], win[j][i], a);
-                        float d = ng[r].get(i);
-                        if (p.silu) d *= silu_grad_of(a, sigmoidf_(a));
-                        if (!INNER) d = u < uend ? d : 0.f;
-                        gp[K - 1][i] = d;
-                        if (INNER || u < t1) {
-                            gb[i] += d;
-#pragma unroll
-                            for (int j = 0; j < K; j++) gw[j][i] = fmaf(d, win[j][i], gw[j][i]);
-                        }
-                        float q = 0.f;
-#pragma unroll
-                        for (int j = 0; j < K; j++) q = fmaf(w[j][i], gp[K - 1 - j][i], q);     // gp of step (u - K + 1) + K - 1 - j
-                        g[i] = q;
-#pragma unroll
-                        for (int j = 0; j < K - 1; j++) { win[j][i] = win[j + 1][i]; gp[j][i] = gp[j + 1][i]; }
+                    for (int j = 0; j < K; j++) a = fma_(w[j], win[j], a);
+                    if (p.silu) {
+                        const Lanes<V> sg = sigmoid_(a);
+                        // silu'(a) = sg (1 + a (1 - sg))
+                        d = mul_(d, mul_(sg, fma_(a, fma_(sg, Lanes<V>::all(-1.f), one), one)));
                     }
-                    const int t = u - (K - 1);
+                    if (!INNER && u >= uend) d = none;
+                    gp[K - 1] = d;
+                    if (INNER || u < t1) {
+                        gb = add_(gb, d);
+#pragma unroll
+                        for (int j = 0; j < K; j++) gw[j] = fma_(d, win[j], gw[j]);
+                    }
+                    Lanes<V> q = mul_(w[0], gp[K - 1]);
+#pragma unroll
+                    for (int j = 1; j < K; j++) q = fma_(w[j], gp[K - 1 - j], q);       // gp of step t + K - 1 - j
+#pragma unroll
+                    for (int j = 0; j < K - 1; j++) { win[j] = win[j + 1]; gp[j] = gp[j + 1]; }
+                    float g[V];
+                    q.get(g);
                     if (INNER || (t >= t0 && t < t1)) store_vec<V>(to + r * p.gx.sL, g);
                 }
             };
@@ -200,11 +240,15 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_bwd_kernel(ConvParams p)
         const float zero[V] = {};
         for (int t = max(t0, t1); t < tend; t++) store_vec<V>(gx + (long long)t * p.gx.sL, zero);
     }
+    float v[V];
+    gb.get(v);
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        red[warp][K][lane * V + i] = gb[i];
+    for (int i = 0; i < V; i++) red[warp][K][lane * V + i] = v[i];
 #pragma unroll
-        for (int j = 0; j < K; j++) red[warp][j][lane * V + i] = gw[j][i];
+    for (int j = 0; j < K; j++) {
+        gw[j].get(v);
+#pragma unroll
+        for (int i = 0; i < V; i++) red[warp][j][lane * V + i] = v[i];
     }
     __syncthreads();
     // partial sums of the CTA: weights as [D][K], then the bias
