@@ -328,20 +328,24 @@ static long long conv_part_rows(int N, int L, int D) {
 }
 
 // ---------------------------------------------------------------- sums of partial gradients
-__global__ void __launch_bounds__(256) column_sums_kernel(ColumnSums p) {
-    __shared__ float red[8][33];
+// 32 columns per CTA, its other threads down the rows: a column of partial sums is as long as the kernel before it had CTAs.  Few columns take
+// 32 rows at a time (592 x 512: 5.6 us, 6.5 with eight), many eight (296 x 20480: 9.7 us, 17.6 with 32: waves of CTAs)
+template <int ROWS>
+__global__ void __launch_bounds__(ROWS * 32) column_sums_kernel(ColumnSums p) {
+    __shared__ float red[ROWS][33];
     griddep_wait();
     griddep_launch_dependents();
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const long long c = (long long)blockIdx.x * 32 + tx;
     float a = 0.f;
     if (c < p.W)
-        for (int r = ty; r < p.P; r += 8) a += p.part[r * p.W + c];
+#pragma unroll 4
+        for (int r = ty; r < p.P; r += ROWS) a += p.part[r * p.W + c];
     red[ty][tx] = a;
     __syncthreads();
     if (ty || c >= p.W) return;
 #pragma unroll
-    for (int i = 1; i < 8; i++) a += red[i][tx];
+    for (int i = 1; i < ROWS; i++) a += red[i][tx];
     long long from = 0;
 #pragma unroll
     for (int k = 0; k < kSumSegments; k++) {
@@ -354,7 +358,9 @@ __global__ void __launch_bounds__(256) column_sums_kernel(ColumnSums p) {
 }
 
 int launch_column_sums(const ColumnSums& p, cudaStream_t st) {
-    return launch_dependent(column_sums_kernel, p, dim3((unsigned)ceil_div(p.W, 32)), 256, 0, st, nullptr);
+    const dim3 grid((unsigned)ceil_div(p.W, 32));
+    if (p.P > 32 && p.W < 32 * 256) return launch_dependent(column_sums_kernel<32>, p, grid, 1024, 0, st, nullptr);
+    return launch_dependent(column_sums_kernel<8>, p, grid, 256, 0, st, nullptr);
 }
 
 }  // namespace fwp

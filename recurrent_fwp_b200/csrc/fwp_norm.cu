@@ -3,84 +3,142 @@
 
 namespace fwp {
 
+// (v - mean) / sd with the mean zero for rms; the variance is taken around the mean
 template <int TPR, int EPT, int V>
-__device__ __forceinline__ void row_statistics(const float (&v)[EPT], const NormParams& p, int tid, float* buf, float& mean, float& rstd) {
-    mean = 0.f;
+__device__ __forceinline__ void row_normalise(f2 (&v)[EPT / 2], const NormParams& p, int tid, float* buf, float& mean, float& rstd) {
     constexpr int W = TPR / 32;
+    mean = 0.f;
     if (!p.rms) {
-        float s[1] = {0.f};
+        f2 a = v[0];
 #pragma unroll
-        for (int i = 0; i < EPT; i++) s[0] += v[i];         // elements beyond the row are zero
+        for (int i = 1; i < EPT / 2; i++) a = fadd2(a, v[i]);
+        float s[1] = {f2_hsum(a)};
         row_sum<TPR, 1>(s, buf);
         mean = s[0] / p.D;
-    }
-    float q[1] = {0.f};
+        const f2 m = f2_all(-mean);
 #pragma unroll
-    for (int i = 0; i < EPT; i++) {
-        const float c = row_has<TPR, V>(i, p.D, tid) ? v[i] - mean : 0.f;
-        q[0] = fmaf(c, c, q[0]);
+        for (int i = 0; i < EPT / 2; i++) v[i] = fadd2(v[i], m);
+        row_cut<TPR, EPT, V>(p.D, tid, v);
     }
-    row_sum<TPR, 1>(q, buf + W);
-    rstd = rsqrtf(q[0] / p.D + p.eps);
+    f2 q = fmul2(v[0], v[0]);
+#pragma unroll
+    for (int i = 1; i < EPT / 2; i++) q = ffma2(v[i], v[i], q);
+    float s[1] = {f2_hsum(q)};
+    row_sum<TPR, 1>(s, buf + W);
+    rstd = rsqrtf(s[0] / p.D + p.eps);
+    const f2 r = f2_all(rstd);
+#pragma unroll
+    for (int i = 0; i < EPT / 2; i++) v[i] = fmul2(v[i], r);
 }
+
+// Rows of more than one warp: a CTA walks rows, the next two on their way to shared memory
+template <typename T, typename TR, int TPR, int EPT, int V>
+struct NormRing {
+    static constexpr int ROW = TPR * EPT, DEPTH = TPR > 32 && V == 4 ? 2 : 0;
+    static constexpr int kGate = ROW * sizeof(T), kRes = 2 * kGate, kStage = kRes + ROW * sizeof(TR);
+    static constexpr size_t bytes = (size_t)DEPTH * kStage;
+};
 
 template <typename T, typename TR, int TPR, int EPT, int V>
 __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) norm_fwd_kernel(NormParams p) {
-    __shared__ float buf[TPR > 32 ? TPR / 32 * 4 : 1];
+    using Ring = NormRing<T, TR, TPR, EPT, V>;
+    constexpr int DEPTH = Ring::DEPTH, RPC = TPR == 32 ? 4 : 1, P = EPT / 2;
+    __shared__ float sums[TPR > 32 ? TPR / 32 * 8 : 1];
+    extern __shared__ float4 norm_smem[];
+    unsigned char* ring = reinterpret_cast<unsigned char*>(norm_smem);
     griddep_wait();
     griddep_launch_dependents();
-    constexpr int RPC = TPR == 32 ? 4 : 1;
     const int tid = threadIdx.x % TPR;
-    const long long row = (long long)blockIdx.x * RPC + threadIdx.x / TPR;
-    if (row >= p.rows) return;
-    const long long n = row / p.L, l = row - n * p.L;
-    auto at = [&](const Stream& s) { return n * s.sN + l * s.sL; };
-    float x[EPT], r[EPT], g[EPT];
-    row_load<TPR, EPT, V>(static_cast<const T*>(p.x.p) + at(p.x), p.D, tid, x);
-    if (p.res.p) row_load<TPR, EPT, V>(static_cast<const TR*>(p.res.p) + at(p.res), p.D, tid, r);
-    if (p.gate.p) row_load<TPR, EPT, V>(static_cast<const T*>(p.gate.p) + at(p.gate), p.D, tid, g);
-    float stats[4] = {0.f, 1.f, 0.f, 1.f};
-    if (p.pw) {
-        row_statistics<TPR, EPT, V>(x, p, tid, buf, stats[0], stats[1]);
-        float w[EPT], b[EPT];
-        row_load<TPR, EPT, V>(p.pw, p.D, tid, w);
-        if (p.pb) row_load<TPR, EPT, V>(p.pb, p.D, tid, b);
+    const long long first = (long long)blockIdx.x * RPC + threadIdx.x / TPR, by = (long long)gridDim.x * RPC;
+    RowAt here(first, DEPTH > 0 ? by : 0, p.L), ahead = here;        // without a ring every row has a warp or CTA of its own
+    auto prefetch = [&](long long row, int stage) {
+        if (row < p.rows) {
+            auto at = [&](const Stream& s) { return ahead.of(s); };
+            unsigned char* to = ring + stage * Ring::kStage;
+            ring_issue<T, TPR, EPT>(to, static_cast<const T*>(p.x.p) + at(p.x), p.D, tid);
+            if (p.gate.p) ring_issue<T, TPR, EPT>(to + Ring::kGate, static_cast<const T*>(p.gate.p) + at(p.gate), p.D, tid);
+            if (p.res.p) ring_issue<TR, TPR, EPT>(to + Ring::kRes, static_cast<const TR*>(p.res.p) + at(p.res), p.D, tid);
+        }
+        cp_async_commit();
+        ahead.next();
+    };
+    if constexpr (DEPTH > 0)
 #pragma unroll
-        for (int i = 0; i < EPT; i++) x[i] = fmaf((x[i] - stats[0]) * stats[1], w[i], p.pb ? b[i] : 0.f);
+        for (int i = 0; i < DEPTH; i++) prefetch(first + i * by, i);
+    int at_stage = 0;
+    for (long long row = first; row < p.rows; row += by, here.next()) {
+        float* buf = sums + (TPR > 32 ? at_stage * (TPR / 8) : 0);      // the rows' sums alternate between two sets of buffers
+        auto at = [&](const Stream& s) { return here.of(s); };
+        f2 x[P], r[P], g[P];
+        if constexpr (DEPTH > 0) cp_async_wait<DEPTH - 1>();
+        const unsigned char* stage = ring + at_stage * Ring::kStage;
+        auto load = [&](auto type, const Stream& s, int offset, auto& v) {
+            using E = decltype(type);
+            if constexpr (DEPTH > 0) row_load<TPR, EPT, V>(reinterpret_cast<const E*>(stage + offset), p.D, tid, v);
+            else row_load<TPR, EPT, V>(static_cast<const E*>(s.p) + at(s), p.D, tid, v);
+        };
+        load(T(), p.x, 0, x);
+        if (p.res.p) load(TR(), p.res, Ring::kRes, r);
+        if (p.gate.p) load(T(), p.gate, Ring::kGate, g);
+        float stats[4] = {0.f, 1.f, 0.f, 1.f};
+        if (p.pw) {
+            row_normalise<TPR, EPT, V>(x, p, tid, buf, stats[0], stats[1]);
+            f2 w[P], b[P];
+            row_load<TPR, EPT, V>(p.pw, p.D, tid, w);
+            if (p.pb) {
+                row_load<TPR, EPT, V>(p.pb, p.D, tid, b);
+#pragma unroll
+                for (int i = 0; i < P; i++) x[i] = ffma2(x[i], w[i], b[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < P; i++) x[i] = fmul2(x[i], w[i]);
+            }
+        }
+        if (p.gate.p) {
+            gate_factor(p.act, g, g);
+#pragma unroll
+            for (int i = 0; i < P; i++) x[i] = fmul2(x[i], g[i]);
+        }
+        if (p.sv) row_load<TPR, EPT, V>(p.sv, p.D, tid, g);
+        else
+#pragma unroll
+            for (int i = 0; i < P; i++) g[i] = f2_all(p.sval);
+        if (p.res.p) {
+#pragma unroll
+            for (int i = 0; i < P; i++) x[i] = ffma2(x[i], g[i], r[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < P; i++) x[i] = fmul2(x[i], g[i]);
+        }
+        row_store<TPR, EPT, V>(static_cast<TR*>(p.r.p) + at(p.r), p.D, tid, x);
+        row_normalise<TPR, EPT, V>(x, p, tid, buf + (TPR > 32 ? TPR / 16 : 0), stats[2], stats[3]);
+        if constexpr (DEPTH > 0) prefetch(row + DEPTH * by, at_stage);      // every value of the stage has been used
+        at_stage ^= 1;
+        row_load<TPR, EPT, V>(p.w, p.D, tid, g);
+        if (p.b) {
+            row_load<TPR, EPT, V>(p.b, p.D, tid, r);
+#pragma unroll
+            for (int i = 0; i < P; i++) x[i] = ffma2(x[i], g[i], r[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < P; i++) x[i] = fmul2(x[i], g[i]);
+        }
+        row_store<TPR, EPT, V>(static_cast<T*>(p.y.p) + at(p.y), p.D, tid, x);
+        if (p.stats && tid == 0) *reinterpret_cast<float4*>(p.stats + 4 * row) = make_float4(stats[0], stats[1], stats[2], stats[3]);
     }
-    if (p.gate.p)
-#pragma unroll
-        for (int i = 0; i < EPT; i++) x[i] *= gate_of(p.act, g[i]);
-    if (p.sv) {
-        row_load<TPR, EPT, V>(p.sv, p.D, tid, g);
-#pragma unroll
-        for (int i = 0; i < EPT; i++) x[i] *= g[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < EPT; i++) x[i] *= p.sval;
-    }
-#pragma unroll
-    for (int i = 0; i < EPT; i++) {
-        if (p.res.p) x[i] += r[i];
-        if (!row_has<TPR, V>(i, p.D, tid)) x[i] = 0.f;
-    }
-    row_store<TPR, EPT, V>(static_cast<TR*>(p.r.p) + at(p.r), p.D, tid, x);
-    row_statistics<TPR, EPT, V>(x, p, tid, buf + (TPR > 32 ? TPR / 16 : 0), stats[2], stats[3]);
-    row_load<TPR, EPT, V>(p.w, p.D, tid, g);
-    if (p.b) row_load<TPR, EPT, V>(p.b, p.D, tid, r);
-#pragma unroll
-    for (int i = 0; i < EPT; i++) x[i] = fmaf((x[i] - stats[2]) * stats[3], g[i], p.b ? r[i] : 0.f);
-    row_store<TPR, EPT, V>(static_cast<T*>(p.y.p) + at(p.y), p.D, tid, x);
-    if (p.stats && tid == 0) *reinterpret_cast<float4*>(p.stats + 4 * row) = make_float4(stats[0], stats[1], stats[2], stats[3]);
 }
 
 template <typename T, typename TR, int TPR, int EPT>
 static int norm_launch(const NormParams& p, bool vec, cudaStream_t st) {
     constexpr int RPC = TPR == 32 ? 4 : 1, threads = TPR == 32 ? 128 : TPR;
-    const long long ctas = ceil_div(p.rows, RPC);
+    long long ctas = ceil_div(p.rows, RPC);
+    if (TPR > 32 && vec) {      // as many CTAs as stay resident: 16 warps and two rows of each are enough for the memory
+        const long long most = (sm_count() > 0 ? sm_count() : 148) * (TPR == 128 ? (EPT == 8 ? 8LL : 4) : TPR == 256 ? 2 : 1);
+        if (ctas > most) ctas = most;
+    }
     if (ctas > 0x7fffffffLL) return FWP_ERR_SHAPE;
-    if (vec) return launch_dependent(norm_fwd_kernel<T, TR, TPR, EPT, 4>, p, dim3((unsigned)ctas), threads, 0, st, "norm_fwd_kernel");
-    return launch_dependent(norm_fwd_kernel<T, TR, TPR, EPT, 1>, p, dim3((unsigned)ctas), threads, 0, st, "norm_fwd_kernel");
+    if (vec) return launch_dependent_beside(norm_fwd_kernel<T, TR, TPR, EPT, 4>, p, dim3((unsigned)ctas), threads, NormRing<T, TR, TPR, EPT, 4>::bytes, st, "norm_fwd_kernel");
+    return launch_dependent_beside(norm_fwd_kernel<T, TR, TPR, EPT, 1>, p, dim3((unsigned)ctas), threads, 0, st, "norm_fwd_kernel");
 }
 template <typename T, typename TR>
 static int norm_dispatch(const NormParams& p, bool vec, cudaStream_t st) {

@@ -59,6 +59,28 @@ static inline bool norm_vectors(const NormParams& p) {
 
 #ifdef __CUDACC__
 
+// Sequence and step of a row, carried from row to row: a 64-bit division per row is as many instructions as the row's arithmetic.
+struct RowAt {
+    long long n, by_n;
+    int l, by_l, L;
+    __device__ __forceinline__ RowAt(long long row, long long by, int L_) : L(L_) {
+        if ((row | by) >> 32) {
+            n = row / L; l = (int)(row - n * L);
+            by_n = by / L; by_l = (int)(by - by_n * L);
+        } else {
+            const unsigned q = (unsigned)row / (unsigned)L, b = (unsigned)by / (unsigned)L;
+            n = q; l = (int)((unsigned)row - q * (unsigned)L);
+            by_n = b; by_l = (int)((unsigned)by - b * (unsigned)L);
+        }
+    }
+    __device__ __forceinline__ void next() {
+        n += by_n;
+        l += by_l;
+        if (l >= L || l < 0) { l -= L; n++; }       // below zero: the sum passed 2^31
+    }
+    __device__ __forceinline__ long long of(const Stream& s) const { return n * s.sN + l * s.sL; }
+};
+
 // sums over the TPR threads of a row; one barrier, the caller alternates `buf`
 template <int TPR, int n>
 __device__ __forceinline__ void row_sum(float (&v)[n], float* buf) {
@@ -83,36 +105,119 @@ __device__ __forceinline__ void row_sum(float (&v)[n], float* buf) {
     }
 }
 
-// a thread's elements of a row: pieces of V, TPR pieces apart
+// a thread's elements of a row, pieces of V that are TPR pieces apart, in pairs for the two-wide instructions; zero beyond the row
 template <int TPR, int EPT, int V, typename T>
-__device__ __forceinline__ void row_load(const T* p, int D, int tid, float (&v)[EPT]) {
+__device__ __forceinline__ void row_load(const T* p, int D, int tid, f2 (&v)[EPT / 2]) {
+    if constexpr (V == 4) {
 #pragma unroll
-    for (int k = 0; k < EPT / V; k++) {
-        const int at = (k * TPR + tid) * V;
-        float q[V] = {};
-        if (at < D) load_vec<V>(p + at, q);
+        for (int k = 0; k < EPT / 4; k++) {
+            const int at = (k * TPR + tid) * 4;
+            float q[4] = {};
+            if (at < D) load_vec<4>(p + at, q);
+            v[2 * k] = f2_pack(q[0], q[1]);
+            v[2 * k + 1] = f2_pack(q[2], q[3]);
+        }
+    } else {
 #pragma unroll
-        for (int i = 0; i < V; i++) v[k * V + i] = q[i];
+        for (int k = 0; k < EPT / 2; k++) {
+            const int at = 2 * k * TPR + tid;
+            v[k] = f2_pack(at < D ? to_f32(p[at]) : 0.f, at + TPR < D ? to_f32(p[at + TPR]) : 0.f);
+        }
     }
 }
 template <int TPR, int EPT, int V, typename T>
-__device__ __forceinline__ void row_store(T* p, int D, int tid, const float (&v)[EPT]) {
+__device__ __forceinline__ void row_store(T* p, int D, int tid, const f2 (&v)[EPT / 2]) {
+    if constexpr (V == 4) {
 #pragma unroll
-    for (int k = 0; k < EPT / V; k++) {
-        const int at = (k * TPR + tid) * V;
-        float q[V];
+        for (int k = 0; k < EPT / 4; k++) {
+            const int at = (k * TPR + tid) * 4;
+            float q[4];
+            f2_unpack(v[2 * k], q[0], q[1]);
+            f2_unpack(v[2 * k + 1], q[2], q[3]);
+            if (at < D) store_vec<4>(p + at, q);
+        }
+    } else {
 #pragma unroll
-        for (int i = 0; i < V; i++) q[i] = v[k * V + i];
-        if (at < D) store_vec<V>(p + at, q);
+        for (int k = 0; k < EPT / 2; k++) {
+            const int at = 2 * k * TPR + tid;
+            float lo, hi;
+            f2_unpack(v[k], lo, hi);
+            if (at < D) p[at] = from_f32<T>(lo);
+            if (at + TPR < D) p[at + TPR] = from_f32<T>(hi);
+        }
     }
 }
-template <int TPR, int V>
-__device__ __forceinline__ bool row_has(int i, int D, int tid) { return ((i / V) * TPR + tid) * V < D; }
+// v with zeros beyond the row, where a mean has been taken off
+template <int TPR, int EPT, int V>
+__device__ __forceinline__ void row_cut(int D, int tid, f2 (&v)[EPT / 2]) {
+    if (D == TPR * EPT) return;
+#pragma unroll
+    for (int k = 0; k < EPT / 2; k++) {
+        if constexpr (V == 4) {
+            v[k] = ((k / 2) * TPR + tid) * 4 < D ? v[k] : 0;
+        } else {
+            float lo, hi;
+            f2_unpack(v[k], lo, hi);
+            const int at = 2 * k * TPR + tid;
+            v[k] = f2_pack(at < D ? lo : 0.f, at + TPR < D ? hi : 0.f);
+        }
+    }
+}
+__device__ __forceinline__ f2 f2_all(float x) { return f2_pack(x, x); }
+__device__ __forceinline__ f2 sigmoid2(f2 x) {
+    float lo, hi;
+    f2_unpack(fmul2(x, f2_all(-kLog2e)), lo, hi);
+    f2_unpack(fadd2(f2_pack(ex2_approx(lo), ex2_approx(hi)), f2_all(1.f)), lo, hi);
+    return f2_pack(rcp_approx(lo), rcp_approx(hi));
+}
+// the gate's factor
+template <int n>
+__device__ __forceinline__ void gate_factor(int act, const f2 (&g)[n], f2 (&a)[n]) {
+    if (act == 2) {
+#pragma unroll
+        for (int i = 0; i < n; i++) a[i] = g[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < n; i++) {
+            const f2 s = sigmoid2(g[i]);
+            a[i] = act == 1 ? s : fmul2(g[i], s);
+        }
+    }
+}
+// the factor, and its derivative in place of the gate
+template <int n>
+__device__ __forceinline__ void gate_factor_and_grad(int act, f2 (&g)[n], f2 (&a)[n]) {
+    const f2 one = f2_all(1.f), minus = f2_all(-1.f);
+    if (act == 2) {
+#pragma unroll
+        for (int i = 0; i < n; i++) { a[i] = g[i]; g[i] = one; }
+    } else if (act == 1) {
+#pragma unroll
+        for (int i = 0; i < n; i++) {
+            a[i] = sigmoid2(g[i]);
+            g[i] = fmul2(a[i], ffma2(a[i], minus, one));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < n; i++) {
+            const f2 s = sigmoid2(g[i]), q = ffma2(s, minus, one);
+            a[i] = fmul2(g[i], s);
+            g[i] = fmul2(s, ffma2(g[i], q, one));
+        }
+    }
+}
 
-__device__ __forceinline__ float gate_of(int act, float g) { return act == 2 ? g : act == 1 ? sigmoidf_(g) : g * sigmoidf_(g); }
-__device__ __forceinline__ float gate_grad_of(int act, float g) {
-    const float s = sigmoidf_(g);
-    return act == 2 ? 1.f : act == 1 ? s * (1.f - s) : silu_grad_of(g, s);
+// The next rows of a thread's streams on their way to shared memory: every thread copies and reads back its own pieces, so the ring needs no
+// barrier.  A row's copy into a stage is issued once the values that were in it have been used.
+template <typename T, int TPR, int EPT>
+__device__ __forceinline__ void ring_issue(unsigned char* stage, const T* row, int D, int tid) {
+#pragma unroll
+    for (int k = 0; k < EPT / 4; k++) {
+        const int at = (k * TPR + tid) * 4;
+        if (at >= D) continue;
+        if constexpr (sizeof(T) == 4) cp_async16(stage + at * 4, row + at);
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(stage + at * 2)), "l"(row + at) : "memory");
+    }
 }
 
 #endif

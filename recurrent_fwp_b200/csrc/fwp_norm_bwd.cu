@@ -11,121 +11,183 @@ namespace fwp {
 
 constexpr int norm_bwd_warps(int TPR) { return TPR == 32 ? 8 : TPR / 32; }
 
+// Rows ahead of the one at work: two where shared memory has room
+template <typename T, typename TR, int TPR, int EPT, int V, bool FULL>
+struct NormBwdRing {
+    static constexpr int SLOTS = TPR == 32 ? 8 : 1, ROW = TPR * EPT;
+    static constexpr int kGy = ROW * sizeof(T), kGate = 2 * kGy, kRes = (FULL ? 3 : 2) * kGy, kGr = kRes + ROW * sizeof(TR), kStage = kGr + ROW * sizeof(TR);
+    static constexpr int kRed = SLOTS > 1 ? SLOTS * ROW * 4 : 0;
+    static constexpr int DEPTH = V != 4 ? 0 : 2 * SLOTS * kStage + kRed <= 230000 ? 2 : 1;
+    static constexpr size_t bytes = (size_t)SLOTS * DEPTH * kStage + kRed;
+};
+
 // FULL: with a norm behind the block, a gate or a scale vector; without, only r = residual + number x
 template <typename T, typename TR, int TPR, int EPT, int V, bool FULL>
 __global__ void __launch_bounds__(norm_bwd_warps(TPR) * 32) norm_bwd_kernel(NormParams p) {
-    constexpr int SLOTS = TPR == 32 ? 8 : 1, NV = FULL ? 5 : 2, W = TPR / 32;
+    constexpr int SLOTS = TPR == 32 ? 8 : 1, NV = FULL ? 5 : 2, W = TPR / 32, P = EPT / 2;
     __shared__ float buf[TPR > 32 ? 8 * W : 1];
-    __shared__ float red[SLOTS > 1 ? SLOTS : 1][SLOTS > 1 ? TPR * EPT : 1];
+    using Ring = NormBwdRing<T, TR, TPR, EPT, V, FULL>;
+    constexpr int DEPTH = Ring::DEPTH;
+    extern __shared__ float4 norm_smem[];
+    float (*red)[TPR * EPT] = reinterpret_cast<float (*)[TPR * EPT]>(norm_smem);
+    unsigned char* ring = reinterpret_cast<unsigned char*>(norm_smem) + Ring::kRed + threadIdx.x / TPR * DEPTH * Ring::kStage;
     griddep_wait();
     griddep_launch_dependents();
     const int tid = threadIdx.x % TPR, slot = threadIdx.x / TPR;
-    float acc[NV][EPT];
+    f2 acc[NV][P];              // sums for weight, bias and, FULL, post_weight, post_bias, scale
 #pragma unroll
     for (int k = 0; k < NV; k++)
 #pragma unroll
-        for (int i = 0; i < EPT; i++) acc[k][i] = 0.f;
+        for (int i = 0; i < P; i++) acc[k][i] = 0;
     const float inv = 1.f / p.D;
-    int par = 0;
-    for (long long row = (long long)blockIdx.x * SLOTS + slot; row < p.rows; row += (long long)gridDim.x * SLOTS, par ^= 1) {
-        const long long n = row / p.L, l = row - n * p.L;
-        auto at = [&](const Stream& s) { return n * s.sN + l * s.sL; };
-        const float4 stats = *reinterpret_cast<const float4*>(p.stats + 4 * row);
-        float x[EPT], r[EPT], g[EPT], gate[FULL ? EPT : 1], sc[FULL ? EPT : 1];
-        row_load<TPR, EPT, V>(static_cast<const T*>(p.x.p) + at(p.x), p.D, tid, x);
+    int par = 0, at_stage = 0;
+    const long long first = (long long)blockIdx.x * SLOTS + slot, by = (long long)gridDim.x * SLOTS;
+    RowAt here(first, by, p.L), ahead = here;
+    auto prefetch = [&](long long row, int stage) {
+        if (row < p.rows) {
+            auto at = [&](const Stream& s) { return ahead.of(s); };
+            unsigned char* to = ring + stage * Ring::kStage;
+            ring_issue<T, TPR, EPT>(to, static_cast<const T*>(p.x.p) + at(p.x), p.D, tid);
+            if (p.gy.p) ring_issue<T, TPR, EPT>(to + Ring::kGy, static_cast<const T*>(p.gy.p) + at(p.gy), p.D, tid);
+            if (FULL && p.gate.p) ring_issue<T, TPR, EPT>(to + Ring::kGate, static_cast<const T*>(p.gate.p) + at(p.gate), p.D, tid);
+            if (p.res.p) ring_issue<TR, TPR, EPT>(to + Ring::kRes, static_cast<const TR*>(p.res.p) + at(p.res), p.D, tid);
+            if (p.gr.p) ring_issue<TR, TPR, EPT>(to + Ring::kGr, static_cast<const TR*>(p.gr.p) + at(p.gr), p.D, tid);
+        }
+        cp_async_commit();
+        ahead.next();
+    };
+    if constexpr (DEPTH > 0)
 #pragma unroll
-        for (int i = 0; i < EPT; i++) r[i] = g[i] = 0.f;
-        if (p.res.p) row_load<TPR, EPT, V>(static_cast<const TR*>(p.res.p) + at(p.res), p.D, tid, r);
-        if (p.gy.p) row_load<TPR, EPT, V>(static_cast<const T*>(p.gy.p) + at(p.gy), p.D, tid, g);
-        float t[FULL ? EPT : 1];        // what the gate multiplies
+        for (int i = 0; i < DEPTH; i++) prefetch(first + i * by, i);
+    float4 next_stats = first < p.rows ? *reinterpret_cast<const float4*>(p.stats + 4 * first) : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (long long row = first; row < p.rows; row += by, par ^= 1, here.next()) {
+        auto at = [&](const Stream& s) { return here.of(s); };
+        const float4 stats = next_stats;
+        if (row + by < p.rows) next_stats = *reinterpret_cast<const float4*>(p.stats + 4 * (row + by));
+        f2 x[P], r[P], g[P], gr[P];
+        if constexpr (DEPTH > 0) cp_async_wait<DEPTH - 1>();
+        const unsigned char* stage = ring + at_stage * Ring::kStage;
+        auto load = [&](auto type, const Stream& s, int offset, auto& v) {
+            using E = decltype(type);
+            if constexpr (DEPTH > 0) row_load<TPR, EPT, V>(reinterpret_cast<const E*>(stage + offset), p.D, tid, v);
+            else row_load<TPR, EPT, V>(static_cast<const E*>(s.p) + at(s), p.D, tid, v);
+        };
+        load(T(), p.x, 0, x);
+#pragma unroll
+        for (int i = 0; i < P; i++) r[i] = g[i] = gr[i] = 0;
+        if (p.res.p) load(TR(), p.res, Ring::kRes, r);
+        if (p.gy.p) load(T(), p.gy, Ring::kGy, g);
+        if (p.gr.p) load(TR(), p.gr, Ring::kGr, gr);
+        // t: what the gate multiplies, a: the gate's factor, da: its derivative, sc: the residual scale
+        f2 t[FULL ? P : 1], a[FULL ? P : 1], da[FULL ? P : 1], sc[FULL ? P : 1], w[P];
         if constexpr (FULL) {
-            if (p.gate.p) row_load<TPR, EPT, V>(static_cast<const T*>(p.gate.p) + at(p.gate), p.D, tid, gate);
-            if (p.sv) row_load<TPR, EPT, V>(p.sv, p.D, tid, sc);
-            else
-#pragma unroll
-                for (int i = 0; i < EPT; i++) sc[i] = p.sval;
             if (p.pw) {
-                row_load<TPR, EPT, V>(p.pw, p.D, tid, t);
-                float b[EPT];
-                if (p.pb) row_load<TPR, EPT, V>(p.pb, p.D, tid, b);
+                const f2 s = f2_all(stats.y), m = f2_all(-stats.x * stats.y);
+                row_load<TPR, EPT, V>(p.pw, p.D, tid, w);
+                if (p.pb) row_load<TPR, EPT, V>(p.pb, p.D, tid, t);
+                else
 #pragma unroll
-                for (int i = 0; i < EPT; i++) {
-                    x[i] = row_has<TPR, V>(i, p.D, tid) ? (x[i] - stats.x) * stats.y : 0.f;
-                    t[i] = fmaf(x[i], t[i], p.pb ? b[i] : 0.f);
+                    for (int i = 0; i < P; i++) t[i] = 0;
+#pragma unroll
+                for (int i = 0; i < P; i++) {
+                    x[i] = ffma2(x[i], s, m);
+                    t[i] = ffma2(x[i], w[i], t[i]);         // zero beyond the row, where w and b are
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < EPT; i++) t[i] = x[i];
+                for (int i = 0; i < P; i++) t[i] = x[i];
             }
+            if (p.gate.p) {
+                load(T(), p.gate, Ring::kGate, da);
+                gate_factor_and_grad(p.act, da, a);
+            } else {
+#pragma unroll
+                for (int i = 0; i < P; i++) a[i] = f2_all(1.f);
+            }
+            if (p.sv) row_load<TPR, EPT, V>(p.sv, p.D, tid, sc);
+            else
+#pragma unroll
+                for (int i = 0; i < P; i++) sc[i] = f2_all(p.sval);
+#pragma unroll
+            for (int i = 0; i < P; i++) r[i] = ffma2(sc[i], fmul2(t[i], a[i]), r[i]);
+        } else {
+            const f2 s = f2_all(p.sval);
+#pragma unroll
+            for (int i = 0; i < P; i++) r[i] = ffma2(s, x[i], r[i]);
         }
-        float s[2] = {0.f, 0.f}, w[EPT];
         row_load<TPR, EPT, V>(p.w, p.D, tid, w);
+        // the mean is taken off before the scaling, as in the forward: r may be large against its spread
+        const f2 rs = f2_all(stats.w), mean = f2_all(-stats.z);
+        f2 s0 = 0, s1 = 0;
 #pragma unroll
-        for (int i = 0; i < EPT; i++) {
-            float u;
-            if constexpr (FULL) u = sc[i] * (p.gate.p ? t[i] * gate_of(p.act, gate[i]) : t[i]);
-            else u = p.sval * x[i];
-            r[i] = row_has<TPR, V>(i, p.D, tid) ? (r[i] + u - stats.z) * stats.w : 0.f;
-            acc[0][i] = fmaf(g[i], r[i], acc[0][i]);
-            acc[1][i] += g[i];
-            g[i] *= w[i];
-            s[0] = fmaf(g[i], r[i], s[0]);
-            s[1] += g[i];
+        for (int i = 0; i < P; i++) {
+            r[i] = fmul2(fadd2(r[i], mean), rs);            // beyond the row g is zero
+            acc[0][i] = ffma2(g[i], r[i], acc[0][i]);
+            acc[1][i] = fadd2(acc[1][i], g[i]);
+            g[i] = fmul2(g[i], w[i]);
+            s0 = ffma2(g[i], r[i], s0);
+            s1 = fadd2(s1, g[i]);
         }
+        float s[2] = {f2_hsum(s0), f2_hsum(s1)};
         row_sum<TPR, 2>(s, buf + par * 4 * W);
-        const float m1 = s[0] * inv, m0 = p.rms ? 0.f : s[1] * inv;
-        if (p.gr.p) row_load<TPR, EPT, V>(static_cast<const TR*>(p.gr.p) + at(p.gr), p.D, tid, w);
+        {
+            const f2 m1 = f2_all(-s[0] * inv), m0 = f2_all(p.rms ? 0.f : -s[1] * inv);
 #pragma unroll
-        for (int i = 0; i < EPT; i++) g[i] = fmaf(stats.w, g[i] - r[i] * m1 - m0, p.gr.p ? w[i] : 0.f);
+            for (int i = 0; i < P; i++) g[i] = ffma2(rs, fadd2(ffma2(r[i], m1, g[i]), m0), gr[i]);
+        }
+        row_cut<TPR, EPT, V>(p.D, tid, g);
+        if constexpr (DEPTH > 0) {              // every value of the stage has been used
+            prefetch(row + DEPTH * by, at_stage);
+            at_stage = at_stage + 1 == DEPTH ? 0 : at_stage + 1;
+        }
         if (p.gres.p) row_store<TPR, EPT, V>(static_cast<TR*>(p.gres.p) + at(p.gres), p.D, tid, g);
         if constexpr (FULL) {
 #pragma unroll
-            for (int i = 0; i < EPT; i++) {
-                const bool in = row_has<TPR, V>(i, p.D, tid);
-                const float a = p.gate.p ? gate_of(p.act, gate[i]) : 1.f;
-                if (in) acc[4][i] = fmaf(g[i], t[i] * a, acc[4][i]);
-                g[i] *= sc[i];
-                if (p.gate.p) gate[i] = g[i] * t[i] * gate_grad_of(p.act, gate[i]);
-                g[i] = in ? g[i] * a : 0.f;
+            for (int i = 0; i < P; i++) {
+                acc[4][i] = ffma2(g[i], fmul2(t[i], a[i]), acc[4][i]);
+                g[i] = fmul2(g[i], sc[i]);
             }
-            if (p.ggate.p) row_store<TPR, EPT, V>(static_cast<T*>(p.ggate.p) + at(p.ggate), p.D, tid, gate);
+            if (p.gate.p) {
+#pragma unroll
+                for (int i = 0; i < P; i++) {
+                    da[i] = fmul2(fmul2(g[i], t[i]), da[i]);
+                    g[i] = fmul2(g[i], a[i]);
+                }
+                row_store<TPR, EPT, V>(static_cast<T*>(p.ggate.p) + at(p.ggate), p.D, tid, da);
+            }
             if (p.pw) {
                 row_load<TPR, EPT, V>(p.pw, p.D, tid, w);
-                s[0] = s[1] = 0.f;
+                s0 = s1 = 0;
 #pragma unroll
-                for (int i = 0; i < EPT; i++) {
-                    acc[2][i] = fmaf(g[i], x[i], acc[2][i]);
-                    acc[3][i] += g[i];
-                    g[i] *= w[i];
-                    s[0] = fmaf(g[i], x[i], s[0]);
-                    s[1] += g[i];
+                for (int i = 0; i < P; i++) {
+                    acc[2][i] = ffma2(g[i], x[i], acc[2][i]);
+                    acc[3][i] = fadd2(acc[3][i], g[i]);
+                    g[i] = fmul2(g[i], w[i]);
+                    s0 = ffma2(g[i], x[i], s0);
+                    s1 = fadd2(s1, g[i]);
                 }
+                s[0] = f2_hsum(s0);
+                s[1] = f2_hsum(s1);
                 row_sum<TPR, 2>(s, buf + par * 4 * W + 2 * W);
-                const float q1 = s[0] * inv, q0 = p.rms ? 0.f : s[1] * inv;
+                const f2 q1 = f2_all(-s[0] * inv), q0 = f2_all(p.rms ? 0.f : -s[1] * inv), ps = f2_all(stats.y);
 #pragma unroll
-                for (int i = 0; i < EPT; i++) g[i] = stats.y * (g[i] - x[i] * q1 - q0);
+                for (int i = 0; i < P; i++) g[i] = fmul2(ps, fadd2(ffma2(x[i], q1, g[i]), q0));
             }
         } else {
+            const f2 sv = f2_all(p.sval);
 #pragma unroll
-            for (int i = 0; i < EPT; i++) g[i] *= p.sval;
+            for (int i = 0; i < P; i++) g[i] = fmul2(g[i], sv);
         }
-        if (p.gx.p) row_store<TPR, EPT, V>(static_cast<T*>(p.gx.p) + at(p.gx), p.D, tid, g);
+        row_store<TPR, EPT, V>(static_cast<T*>(p.gx.p) + at(p.gx), p.D, tid, g);
     }
     float* part = p.part + (long long)blockIdx.x * p.D * NV;
-    if constexpr (SLOTS == 1) {
 #pragma unroll
-        for (int k = 0; k < NV; k++)
-#pragma unroll
-            for (int i = 0; i < EPT; i++) {
-                const int c = ((i / V) * TPR + tid) * V + i % V;
-                if (c < p.D) part[(long long)k * p.D + c] = acc[k][i];
-            }
-    } else {
-#pragma unroll
-        for (int k = 0; k < NV; k++) {
+    for (int k = 0; k < NV; k++) {
+        if constexpr (SLOTS == 1) {
+            row_store<TPR, EPT, V>(part + (long long)k * p.D, p.D, tid, acc[k]);
+        } else {
             __syncthreads();
-#pragma unroll
-            for (int i = 0; i < EPT; i++) red[slot][((i / V) * TPR + tid) * V + i % V] = acc[k][i];
+            row_store<TPR, EPT, V>(red[slot], p.D, tid, acc[k]);
             __syncthreads();
             for (int c = threadIdx.x; c < p.D; c += SLOTS * TPR) {
                 float a = 0.f;
@@ -137,10 +199,10 @@ __global__ void __launch_bounds__(norm_bwd_warps(TPR) * 32) norm_bwd_kernel(Norm
     }
 }
 
-// CTAs: enough warps to keep the memory busy, and no more partial sums than that
-static int norm_bwd_ctas(long long rows, int D) {
+// CTAs: as many as registers let stay resident, and no more partial sums than that
+static int norm_bwd_ctas(long long rows, int D, bool full) {
     const long long sms = sm_count() > 0 ? sm_count() : 148;
-    const long long per_sm = D <= 1024 ? 4 : D <= 2048 ? 3 : D <= 4096 ? 2 : 1;
+    const long long per_sm = D <= 256 ? (full ? 1 : 2) : D <= 512 ? (full ? 6 : 12) : D <= 1024 ? (full ? 3 : 6) : D <= 2048 ? (full ? 1 : 3) : 1;
     const long long most = D <= 256 ? ceil_div(rows, 8) : rows;
     return (int)(most < sms * per_sm ? most : sms * per_sm);
 }
@@ -148,8 +210,9 @@ static int norm_bwd_ctas(long long rows, int D) {
 template <typename T, typename TR, int TPR, int EPT, bool FULL>
 static int norm_bwd_launch(const NormParams& p, bool vec, int ctas, cudaStream_t st) {
     constexpr int threads = norm_bwd_warps(TPR) * 32;
-    if (vec) return launch_dependent(norm_bwd_kernel<T, TR, TPR, EPT, 4, FULL>, p, dim3(ctas), threads, 0, st, "norm_bwd_kernel");
-    return launch_dependent(norm_bwd_kernel<T, TR, TPR, EPT, 1, FULL>, p, dim3(ctas), threads, 0, st, "norm_bwd_kernel");
+    constexpr size_t b4 = NormBwdRing<T, TR, TPR, EPT, 4, FULL>::bytes, b1 = NormBwdRing<T, TR, TPR, EPT, 1, FULL>::bytes;
+    if (vec) return launch_dependent_beside(norm_bwd_kernel<T, TR, TPR, EPT, 4, FULL>, p, dim3(ctas), threads, b4, st, "norm_bwd_kernel");
+    return launch_dependent_beside(norm_bwd_kernel<T, TR, TPR, EPT, 1, FULL>, p, dim3(ctas), threads, b1, st, "norm_bwd_kernel");
 }
 template <typename T, typename TR, bool FULL>
 static int norm_bwd_dispatch(const NormParams& p, bool vec, int ctas, cudaStream_t st) {
@@ -167,7 +230,8 @@ using namespace fwp;
 
 FWP_API int64_t fwp_block_norm_backward_scratch_floats(int N, int L, int D) {
     if (N <= 0 || L <= 0 || D <= 0 || D > kNormMaxD) return 0;
-    return (int64_t)norm_bwd_ctas((long long)N * L, D) * D * 5;
+    const long long rows = (long long)N * L;
+    return (int64_t)(norm_bwd_ctas(rows, D, true) > norm_bwd_ctas(rows, D, false) ? norm_bwd_ctas(rows, D, true) : norm_bwd_ctas(rows, D, false)) * D * 5;
 }
 
 FWP_API int fwp_block_norm_backward(int N, int L, int D, const fwp_tensor* x, const fwp_tensor* residual, const fwp_tensor* gate,
@@ -208,7 +272,7 @@ FWP_API int fwp_block_norm_backward(int N, int L, int D, const fwp_tensor* x, co
     for (const Stream* s : {&p.x, &p.gate, &p.gy, &p.gx, &p.ggate}) vec = vec && rows_aligned(*s, esz, 4 * esz);
     for (const Stream* s : {&p.res, &p.gr, &p.gres}) vec = vec && rows_aligned(*s, rsz, 4 * rsz);
     const bool full = p.pw || p.gate.p || p.sv;
-    const int ctas = norm_bwd_ctas(p.rows, D);
+    const int ctas = norm_bwd_ctas(p.rows, D, full);
     auto run = [&](auto t, auto r) {
         using T = decltype(t);
         using TR = decltype(r);

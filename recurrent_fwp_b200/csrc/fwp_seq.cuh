@@ -37,6 +37,16 @@ struct ColumnSums {
 };
 int launch_column_sums(const ColumnSums& p, cudaStream_t st);
 
+// launch_dependent for kernels with static shared memory beside the dynamic: the two together may pass 48 KB
+template <typename K, typename P>
+static int launch_dependent_beside(K kern, const P& p, dim3 grid, int threads, size_t bytes, cudaStream_t st, const char* name) {
+    if (bytes > 32 * 1024) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e != cudaSuccess) return set_cuda_error(e);
+    }
+    return launch_dependent(kern, p, grid, threads, bytes, st, name);
+}
+
 #ifdef __CUDACC__
 
 __device__ __forceinline__ f2 fmul2(f2 a, f2 b) {
