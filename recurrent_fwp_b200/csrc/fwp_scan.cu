@@ -31,8 +31,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 3) scan_fwd_kernel(ScanParams
     constexpr int CW = Tile::CW, OS = Tile::OS, TT = Tile::TT, S4 = Tile::S4, NT = kScanWarps * 32;
     constexpr bool WHOLE = PASS == SCAN_WHOLE;
     __shared__ __align__(16) Tile sm;
-    griddep_wait();
-    griddep_launch_dependents();
+    griddep_wait();         // and no early launch of the next kernel: its CTAs would take this one's places unevenly (a prompt of 16384: 448 -> 621 us)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int grp = lane / LPC, j = lane % LPC;             // two channels; their states 4 j ... 4 j + 3, their steps j, j + LPC ...
     const int n = blockIdx.z, span = blockIdx.y;
@@ -205,7 +204,6 @@ struct ScanJoinParams {
 __global__ void __launch_bounds__(256) scan_join_kernel(ScanJoinParams q) {
     const ScanParams& p = q.p;
     griddep_wait();
-    griddep_launch_dependents();
     const long long e = (long long)blockIdx.x * 256 + threadIdx.x, per_seq = (long long)p.D * p.S;
     if (e >= per_seq) return;
     const int n = blockIdx.y, d = (int)(e / p.S), s = (int)(e - (long long)d * p.S);

@@ -54,7 +54,6 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 2) scan_bwd_kernel(ScanParams 
     constexpr bool WHOLE = PASS == SCAN_WHOLE;
     __shared__ __align__(16) Tile sm;
     griddep_wait();
-    griddep_launch_dependents();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int grp = lane / LPC, j = lane % LPC;
     const int n = blockIdx.z, span = WHOLE ? blockIdx.y : blockIdx.y + 1;       // nothing in front of the first span asks for its end
