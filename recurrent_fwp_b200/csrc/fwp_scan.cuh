@@ -17,7 +17,7 @@ struct ScanParams {
     const int* lengths;
     float* state;           // (N, D, S), null: zeros
     long long state_sN, state_sD;
-    bool state_vec;         // rows of the state move in 16-byte pieces
+    bool state_vec;         // a single step moves rows of the state, of B and of C in pieces of four
     bool pairs;             // the rows of two neighbouring channels move as one
     float* checkpoints;     // [N][ceil(L / 8)][D][scan_row(S)]
     float *ends, *dsums;    // [N][spans][D][S] and [N][spans][D]
