@@ -328,7 +328,7 @@ static ScanPlan scan_plan(int N, int L, int D, int S, int G) {
     if (forced > 0) spans = ceil_div(L, ceil_div(forced, tile) * tile);
     else if (ctas * 3 <= sms * 2) {
         spans = sms * 2 / ctas;
-        const long long most = ceil_div(L, 4 * tile);
+        const long long most = ceil_div(L, 2 * tile);
         if (spans > most) spans = most;
     }
     if (spans > 4096) spans = 4096;

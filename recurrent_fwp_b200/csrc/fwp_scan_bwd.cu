@@ -463,7 +463,7 @@ static ScanBwdPlan scan_bwd_plan(int N, int L, int D, int S, int G) {
     const int forced = tune_get(T_SCAN_CHUNK, 0);
     int spans = 1;
     if (forced > 0) spans = (int)ceil_div(L, ceil_div(forced, kScanKeep) * kScanKeep);
-    else if (ctas * 3 <= sms * 2) spans = (int)(sms * 2 / ctas);
+    else if (ctas <= sms) spans = (int)(sms * 2 / ctas);
     const int most = (int)ceil_div(L, 8 * kScanKeep);
     if (!forced && spans > most) spans = most;
     if (spans > 4096) spans = 4096;
