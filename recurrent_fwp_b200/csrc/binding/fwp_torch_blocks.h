@@ -98,7 +98,8 @@ Tensor rows_as(const Tensor& x, at::ScalarType type) {
     }
     return empty({x.size(0), x.size(1)}, type, x);
 }
-Tensor vector_for(const Tensor& w) { return w.defined() ? at::empty(w.sizes(), w.options()) : Tensor(); }
+Tensor empty_as(const Tensor& t) { return Tensor(at::detail::empty_cuda(t.sizes(), t.scalar_type(), t.device(), std::nullopt)); }
+Tensor vector_for(const Tensor& w) { return w.defined() ? empty_as(w) : Tensor(); }
 Tensor scratch_of(int64_t n, const Tensor& like) { return n > 0 ? empty({n}, at::kFloat, like) : Tensor(); }
 int flag(PyObject* o) { return PyObject_IsTrue(o); }
 
@@ -172,7 +173,7 @@ struct ScanNode final : public OpNode {
         if (z.defined()) gz = rows_as(z, x.scalar_type());
         Tensor gA = vector_for(A), gB, gC, gskip = vector_for(skip),
                gbias = vector_for(bias);
-        for (Tensor* q : {&gB, &gC}) *q = x.numel() ? at::empty(B.sizes(), B.options()) : at::zeros(B.sizes(), B.options());
+        for (Tensor* q : {&gB, &gC}) *q = x.numel() ? empty_as(B) : at::zeros(B.sizes(), B.options());
         const int64_t need = fwp_selective_scan_backward_scratch_floats(N, L, D, S, G, dev);
         const Tensor scratch = scratch_of(need, x);
         check(fwp_selective_scan_backward(N, L, D, S, G, RowsDesc(x), RowsDesc(dt), floats(A), GroupDesc(B), GroupDesc(C), floats(skip), RowsDesc(z),

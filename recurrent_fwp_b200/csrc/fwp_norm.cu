@@ -72,14 +72,20 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) norm_fwd_kernel(NormPar
         f2 x[P], r[P], g[P];
         if constexpr (DEPTH > 0) cp_async_wait<DEPTH - 1>();
         const unsigned char* stage = ring + at_stage * Ring::kStage;
-        auto load = [&](auto type, const Stream& s, int offset, auto& v) {
-            using E = decltype(type);
-            if constexpr (DEPTH > 0) row_load<TPR, EPT, V>(reinterpret_cast<const E*>(stage + offset), p.D, tid, v);
-            else row_load<TPR, EPT, V>(static_cast<const E*>(s.p) + at(s), p.D, tid, v);
-        };
-        load(T(), p.x, 0, x);
-        if (p.res.p) load(TR(), p.res, Ring::kRes, r);
-        if (p.gate.p) load(T(), p.gate, Ring::kGate, g);
+        if constexpr (DEPTH > 0) {
+            row_load<TPR, EPT, V>(reinterpret_cast<const T*>(stage), p.D, tid, x);
+            if (p.res.p) row_load<TPR, EPT, V>(reinterpret_cast<const TR*>(stage + Ring::kRes), p.D, tid, r);
+            if (p.gate.p) row_load<TPR, EPT, V>(reinterpret_cast<const T*>(stage + Ring::kGate), p.D, tid, g);
+        } else {
+            RawVec<T, V> rx[EPT / V], rg[EPT / V];
+            RawVec<TR, V> rr[EPT / V];
+            row_fetch<TPR, EPT, V>(static_cast<const T*>(p.x.p) + at(p.x), true, p.D, tid, rx);
+            row_fetch<TPR, EPT, V>(static_cast<const TR*>(p.res.p) + at(p.res), p.res.p != nullptr, p.D, tid, rr);
+            row_fetch<TPR, EPT, V>(static_cast<const T*>(p.gate.p) + at(p.gate), p.gate.p != nullptr, p.D, tid, rg);
+            row_convert<EPT, V>(rx, x);
+            row_convert<EPT, V>(rr, r);
+            row_convert<EPT, V>(rg, g);
+        }
         float stats[4] = {0.f, 1.f, 0.f, 1.f};
         if (p.pw) {
             row_normalise<TPR, EPT, V>(x, p, tid, buf, stats[0], stats[1]);

@@ -125,6 +125,21 @@ __device__ __forceinline__ void row_load(const T* p, int D, int tid, f2 (&v)[EPT
         }
     }
 }
+// the same in two steps, so that the loads of several streams are under way before the first is converted
+template <int TPR, int EPT, int V, typename T>
+__device__ __forceinline__ void row_fetch(const T* p, bool on, int D, int tid, RawVec<T, V> (&raw)[EPT / V]) {
+#pragma unroll
+    for (int k = 0; k < EPT / V; k++) {
+        const int at = (k * TPR + tid) * V;
+        raw[k].clear();
+        if (on && at < D) raw[k].load(p + at);
+    }
+}
+template <int EPT, int V, typename T>
+__device__ __forceinline__ void row_convert(const RawVec<T, V> (&raw)[EPT / V], f2 (&v)[EPT / 2]) {
+#pragma unroll
+    for (int i = 0; i < EPT / 2; i++) v[i] = f2_pack(raw[2 * i / V].get(2 * i % V), raw[(2 * i + 1) / V].get((2 * i + 1) % V));
+}
 template <int TPR, int EPT, int V, typename T>
 __device__ __forceinline__ void row_store(T* p, int D, int tid, const f2 (&v)[EPT / 2]) {
     if constexpr (V == 4) {

@@ -97,16 +97,19 @@ __device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float (&v)[V])
 template <typename T, int V> struct RawVec;
 template <typename T> struct RawVec<T, 1> {
     T v;
+    __device__ __forceinline__ void clear() { v = from_f32<T>(0.f); }
     __device__ __forceinline__ void load(const T* p) { v = *p; }
     __device__ __forceinline__ float get(int) const { return to_f32(v); }
 };
 template <> struct RawVec<float, 4> {
     float4 v;
+    __device__ __forceinline__ void clear() { v = make_float4(0.f, 0.f, 0.f, 0.f); }
     __device__ __forceinline__ void load(const float* p) { v = *reinterpret_cast<const float4*>(p); }
     __device__ __forceinline__ float get(int i) const { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 };
 template <> struct RawVec<__nv_bfloat16, 4> {
     uint2 v;
+    __device__ __forceinline__ void clear() { v = make_uint2(0u, 0u); }
     __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = *reinterpret_cast<const uint2*>(p); }
     __device__ __forceinline__ float get(int i) const {
         const unsigned w = i < 2 ? v.x : v.y;
