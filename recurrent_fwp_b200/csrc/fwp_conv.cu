@@ -5,8 +5,10 @@
 //
 // Bound by the bytes: forward one element in and one out per (n, t, d), backward two in and one out.  A warp owns 32 x V channels
 // of one sequence and walks a span of steps with the last K - 1 inputs in registers, so every input is read once (and K - 1 of
-// a neighbour's span, from L2); eight rows are in flight per warp.  The backward walks forwards too: it forms p again from
-// the inputs it needs for gw anyway, and gx K - 1 steps behind.
+// a neighbour's span, from L2); a block of four to eight rows is on its way while the one before it is worked on.  More rows in flight
+// cost registers and with them warps: of 2 to 16 rows and 3 to 8 CTAs per SM these were the fastest (8 x 2048 x 2048, bf16, 4 taps: 31 us
+// forward, 4.3 TB/s, and 55 us backward, 3.7 TB/s).  The backward walks forwards too: it forms p again from the inputs it needs
+// for gw anyway, and gx K - 1 steps behind.
 #include <type_traits>
 #include "fwp_seq.cuh"
 

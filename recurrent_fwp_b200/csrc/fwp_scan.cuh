@@ -5,9 +5,9 @@
 namespace fwp {
 
 constexpr int kScanMaxS = 64;
-// The forward of a call with a backward keeps the state before every eighth step.  The backward then forms exp(delta A) once per
-// state and step, and holds a tile's states and decays in registers; farther apart it would have to form them twice, and the
-// exponentials are what bounds both directions.  8 bytes per (step, channel) each way at S = 16.
+// The forward of a call with a backward keeps the state before every eighth step: 8 bytes per (step, channel) each way at S = 16, beside
+// about 8 and 14 of streams in bf16.  The backward holds half a tile's states and decays in registers and forms the first half's twice; from
+// states kept farther apart it would form all of them once more.
 constexpr int kScanKeep = 8;
 
 struct ScanParams {
