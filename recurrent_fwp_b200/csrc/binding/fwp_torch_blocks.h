@@ -24,14 +24,15 @@ bool any_needs_grad(const std::array<const Tensor*, K>& in) {
         if (t && t->requires_grad()) return true;
     return false;
 }
+// A state is not saved: no backward reads it, and its owner may overwrite it before.
 template <class NodeT, size_t K>
-std::shared_ptr<NodeT> optional_node(const std::array<const Tensor*, K>& in) {
+std::shared_ptr<NodeT> optional_node(const std::array<const Tensor*, K>& in, size_t state = K) {
     auto node = std::shared_ptr<NodeT>(new NodeT(), torch::autograd::deleteNode);
     torch::autograd::edge_list edges;
     edges.reserve(K);
     for (auto* t : in) edges.push_back(t && t->requires_grad() ? torch::autograd::impl::gradient_edge(*t) : torch::autograd::Edge());
     node->set_next_edges(std::move(edges));
-    for (auto* t : in) node->save(t ? *t : Tensor());
+    for (size_t i = 0; i < K; i++) node->save(in[i] && i != state ? *in[i] : Tensor());
     return node;
 }
 
@@ -147,7 +148,7 @@ PyObject* causal_conv(PyObject*, PyObject* const* args, Py_ssize_t n) {
         check(fwp_causal_conv_forward(N, L, D, K, RowsDesc(x), floats(&w), floats(in[2]), RowsDesc(K > 1 ? in[3] : nullptr), ints(in[4]),
                                       RowsDesc(out), silu, dtype_code(x), stream_of(x), dev.index()), "causal_conv_forward");
         if (grad) {
-            auto node = optional_node<ConvNode>(in);
+            auto node = optional_node<ConvNode>(in, 3);
             node->silu = silu;
             node->keep({start});
             torch::autograd::create_gradient_edge(out, node);
@@ -222,7 +223,7 @@ PyObject* selective_scan(PyObject*, PyObject* const* args, Py_ssize_t n) {
                                          RowsDesc(in[6]), floats(in[7]), RowsDesc(in[8]), ints(in[9]), RowsDesc(out), floats(keep),
                                          floats(scratch), need, softplus, dtype_code(x), stream_of(x), dev.index()), "selective_scan_forward");
         if (grad) {
-            auto node = optional_node<ScanNode>(in);
+            auto node = optional_node<ScanNode>(in, 8);
             node->softplus = softplus;
             node->keep({keep});
             torch::autograd::create_gradient_edge(out, node);

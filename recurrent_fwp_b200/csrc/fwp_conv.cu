@@ -279,7 +279,7 @@ static int conv_check(int N, int L, int D, int K, const fwp_tensor* x, const flo
     if (N < 0 || L < 0 || D < 0 || K < 1) return FWP_ERR_SHAPE;
     if (io_dtype != FWP_F32 && io_dtype != FWP_BF16) return FWP_ERR_DTYPE;
     if (K > kConvMaxK) return FWP_ERR_UNSUPPORTED;
-    if (N > 65535) return FWP_ERR_SHAPE;
+    if (N > 65535 || L > kMaxSteps) return FWP_ERR_SHAPE;
     if (D && !w) return FWP_ERR_NULL;
     if (!aligned4(w) || !aligned4(b) || !aligned4(lengths)) return FWP_ERR_ALIGN;
     if (!N || !L || !D) return FWP_OK;

@@ -44,7 +44,7 @@ static inline int scan_row(int S) { return (S + 3) & ~3; }
 static inline int scan_check(int N, int L, int D, int S, int G, const fwp_tensor* x, const fwp_tensor* dt, const float* A,
                              const fwp_tensor* B, const fwp_tensor* C, const float* skip, const fwp_tensor* z, const float* dt_bias,
                              const int* lengths, int io_dtype) {
-    if (N < 0 || L < 0 || D < 0 || S < 1 || G < 1 || D % G || N > 65535) return FWP_ERR_SHAPE;
+    if (N < 0 || L < 0 || D < 0 || S < 1 || G < 1 || D % G || N > 65535 || L > kMaxSteps) return FWP_ERR_SHAPE;
     if (io_dtype != FWP_F32 && io_dtype != FWP_BF16) return FWP_ERR_DTYPE;
     if (S > kScanMaxS) return FWP_ERR_UNSUPPORTED;
     if (D && !A) return FWP_ERR_NULL;
@@ -83,7 +83,7 @@ __device__ __forceinline__ float softplus_(float x) {
     r = fmaf(r, q, 1.f / 5.f);
     r = fmaf(r, q, 1.f / 3.f);
     r = fmaf(r, q, 1.f);
-    return fmaf(2.f * s, r, x > 0.f ? x : 0.f * x);     // 0 x keeps a NaN
+    return fmaf(2.f * s, r, fmaxf(x, 0.f));     // a NaN is in s
 }
 
 __device__ __forceinline__ f2 exp2_pair(f2 v) {

@@ -23,6 +23,8 @@ static inline bool rows_aligned(const Stream& s, int esz, int bytes) {
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 static inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 
+constexpr int kMaxSteps = 0x7fff0000;       // of a sequence: the step behind a span's end is an int
+
 static inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 // Sums over the rows of part[P][W], columns cut into segments that go to tensors of their own (null: not wanted).  The order of

@@ -68,6 +68,7 @@ def test_against_the_definition(fwp, shape, dtype):
     N, L, D, S, G = shape
     check(fwp, *make(1, N, L, D, S, G, dtype))
     check(fwp, *make(2, N, L, D, S, G, dtype, layout='sliced', lengths='inside'))
+    check(fwp, *make(22, N, L, D, S, G, dtype, layout='expanded'))
 
 
 @pytest.mark.parametrize('leave_out', ['z', 'skip', 'bias', 'state', 'all'])
@@ -123,6 +124,17 @@ def test_extreme_step_sizes(fwp):
     fwp.selective_scan(**dict(a, x=a['x'][:, :1], dt=a['dt'][:, :1], B=a['B'][:, :1], C=a['C'][:, :1], state=state))
     # h = log(1 + e^-18), to 64 U of itself
     assert ((state.double() / torch.log1p(torch.exp(torch.tensor(-18., dtype=torch.float64))).item()) - 1).abs().max() < 64 * 2.0 ** -24
+
+
+def test_step_sizes_of_minus_infinity_leave_the_state(fwp):
+    a, gy = make(21, 2, 12, 40, 16, bias=False)
+    for L in (12, 1):
+        b = {k: t[:, :L].clone() if k in ('x', 'dt', 'z', 'B', 'C') else t for k, t in a.items()}
+        b['dt'][0] = -float('inf')
+        b['dt'][1, :, :20] = torch.finfo(F32).min
+        out, state, grads = run(fwp, b, gy[:, :L])
+        assert torch.equal(state[0], a['state'][0]) and torch.equal(state[1, :20], a['state'][1, :20])
+        assert torch.isfinite(out).all() and not grads['dt'][0].any() and all(torch.isfinite(g).all() for g in grads.values())
 
 
 def test_lengths_outside_the_range_and_as_int64(fwp):

@@ -240,6 +240,26 @@ def test_tracing_and_transforms(fwp, name):
         torch.func.grad(lambda t: call(t, *leaves[1:]).sum())(leaves[0])
 
 
+@pytest.mark.parametrize('name', ['conv', 'scan'])
+def test_a_state_overwritten_before_the_backward(fwp, name):
+    """No backward reads the state: a caller may reset it, or go on with the next segment, first."""
+    a = arguments(14, 2, 40, 32, grad=True)
+    window, state = (torch.randn_like(m) for m in memories(2, 32))
+
+    def call():
+        if name == 'conv':
+            m = window.clone()
+            return m, fwp.causal_conv(a['x'], a['w'], a['b'], state=m), [a['x'], a['w'], a['b']]
+        m = state.clone()
+        leaves = [a[k] for k in ('x', 'dt', 'A', 'B', 'C')]
+        return m, fwp.selective_scan(*leaves, state=m), leaves
+    m, y, leaves = call()
+    ref = torch.autograd.grad(y.sum(), leaves)
+    m, y, leaves = call()
+    m.fill_(float('nan'))
+    assert all(torch.equal(p, q) for p, q in zip(ref, torch.autograd.grad(y.sum(), leaves)))
+
+
 def test_undefined_and_partial_gradients(fwp):
     """Leaves that need no gradient, outputs that nobody uses, gradients of another type."""
     a = arguments(13, 2, 30, 32, dtype=BF16)
