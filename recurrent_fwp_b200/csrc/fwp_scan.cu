@@ -8,7 +8,7 @@
 // lane with the value of one step; that lane loads x, dt, z for it and stores its output, so y goes through no memory.
 //
 // The exponentials bound it: S per (step, channel), 16 a clock and SM.  At 8 x 2048 x 2048 (bf16, S = 16) that is 115 us, and 29 us more for
-// softplus and silu; measured 290 us, 325 us with checkpoints.  With one channel per lane shared memory was the limit (B and C read for 8
+// softplus and silu; measured 290 us, 321 us with checkpoints.  With one channel per lane shared memory was the limit (B and C read for 8
 // channels at a time, 89 % of the pipe, 383 us); with two it is the latency of 1.7 warps per scheduler (exponential unit 48 %, issue 47 %).
 #include "fwp_scan.cuh"
 
@@ -30,7 +30,7 @@ struct ScanTile {
 // One span of time of one warp's channels.  PASS = SCAN_ENDS: only the state that the span leaves behind, starting from zero, and
 // the sum of delta, for joining spans (scan_join_kernel).
 template <typename T, int LPC, bool RAGGED, bool PAIRS, int PASS>
-__global__ void __launch_bounds__(kScanWarps * 32, 3) scan_fwd_kernel(ScanParams p) {
+__global__ void __launch_bounds__(kScanWarps * 32, PASS == SCAN_WHOLE ? 4 : 3) scan_fwd_kernel(ScanParams p) {
     using Tile = ScanTile<LPC>;
     constexpr int CW = Tile::CW, OS = Tile::OS, TT = Tile::TT, S4 = Tile::S4, NT = kScanWarps * 32;
     constexpr bool WHOLE = PASS == SCAN_WHOLE;
@@ -328,7 +328,7 @@ static ScanPlan scan_plan(int N, int L, int D, int S, int G) {
     const long long sms = sm_count() > 0 ? sm_count() : 148, ctas = (long long)N * G * ceil_div(D / G, cta);
     const int forced = tune_get(T_SCAN_CHUNK, 0);
     long long spans = 1;
-    // Spans side by side form the exponentials of a step twice, so they have to bring more than twice the CTAs, of which an SM holds two to three.
+    // Spans side by side form the exponentials of a step twice, so they have to bring more than twice the CTAs, of which an SM holds four and is busy with two.
     if (forced > 0) spans = ceil_div(L, ceil_div(forced, tile) * tile);
     else if (ctas * 3 <= sms * 2) {
         spans = sms * 2 / ctas;
