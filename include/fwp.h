@@ -445,7 +445,7 @@ int fwp_selective_scan_backward(int N, int L, int D, int S, int G, const fwp_ten
  *   t = post_weight ? norm(x; post_weight, post_bias) : x,   u = gate ? t act(gate) : t
  *   r = residual + scale u,   y = norm(r; weight, bias)
  *   norm(v; w, b) = (v - mean v) / sqrt(var v + eps) w + b,  with rms: v / sqrt(mean v^2 + eps) w
- * gate_act 0: act(g) = g silu-wise (g sigmoid(g)), 1: sigmoid(g), 2: g.  scale: scale_vector [D], or the number scale_value where
+ * gate_act 0: act(g) = g sigmoid(g), 1: sigmoid(g), 2: g.  scale: scale_vector [D], or the number scale_value where
  * that is NULL.  residual, gate: data == NULL for none.  y has x's element type; residual and r have residual_dtype, which is
  * io_dtype or FWP_F32.  stats (may be NULL when no backward follows): N*L*4 floats. */
 int fwp_block_norm_forward(int N, int L, int D, const fwp_tensor* x, const fwp_tensor* residual, const fwp_tensor* gate,

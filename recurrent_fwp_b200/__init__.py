@@ -5,6 +5,8 @@ Sub-packages carry the reference's module names so that its layer code imports
 them unchanged: ``fast_weight`` (delta rule), ``fast_transformers`` (sum rule),
 ``rec_update_fwm_tanh``, ``fast_weight_rnn_v2``, ``fast_weight_rnn``,
 ``fast_lstm``, ``fast_lstm_v2``, ``fast_lstm_v3``, ``fast_lstm_v4``.
+Beside them stand the operators of a state-space layer, which the reference
+does not have: ``causal_conv``, ``selective_scan``, ``block_norm``.
 Importing this package loads ``libfwp.so``; it raises if the library has not
 been built (there is no CPU path).
 """
@@ -25,4 +27,4 @@ from .block_norm import block_norm  # noqa: F401
 __all__ = ['DeltaFastWeight', 'fast_weight_delta', 'FastWeightSum', 'fast_weight_sum',
            'FastWeightRecUpdateTanh', 'rec_update_fwm_tanh', 'FastRNNv2', 'fast_rnn_v2', 'FastRNN', 'fast_rnn',
            'FastLSTM', 'fast_lstm', 'FastLSTMv2', 'fast_lstm_v2', 'FastLSTMv3', 'fast_lstm_v3',
-           'FastLSTMv4', 'fast_lstm_v4']
+           'FastLSTMv4', 'fast_lstm_v4', 'causal_conv', 'selective_scan', 'block_norm']

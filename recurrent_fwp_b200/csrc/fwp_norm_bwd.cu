@@ -10,6 +10,10 @@
 namespace fwp {
 
 constexpr int norm_bwd_warps(int TPR) { return TPR == 32 ? 8 : TPR / 32; }
+// CTAs that an SM is to hold: 24 warps of the short forms with two sums per element, 16 with five, fewer of the long rows'
+constexpr int norm_bwd_resident(int TPR, int EPT, bool FULL) {
+    return TPR == 32 ? 2 : EPT == 4 || (EPT == 8 && !FULL) ? 24 / norm_bwd_warps(TPR) : EPT == 8 || !FULL ? 16 / norm_bwd_warps(TPR) : 1;
+}
 
 // Rows ahead of the one at work: two where shared memory has room
 template <typename T, typename TR, int TPR, int EPT, int V, bool FULL>
@@ -23,7 +27,7 @@ struct NormBwdRing {
 
 // FULL: with a norm behind the block, a gate or a scale vector; without, only r = residual + number x
 template <typename T, typename TR, int TPR, int EPT, int V, bool FULL>
-__global__ void __launch_bounds__(norm_bwd_warps(TPR) * 32) norm_bwd_kernel(NormParams p) {
+__global__ void __launch_bounds__(norm_bwd_warps(TPR) * 32, norm_bwd_resident(TPR, EPT, FULL)) norm_bwd_kernel(NormParams p) {
     constexpr int SLOTS = TPR == 32 ? 8 : 1, NV = FULL ? 5 : 2, W = TPR / 32, P = EPT / 2;
     __shared__ float buf[TPR > 32 ? 8 * W : 1];
     using Ring = NormBwdRing<T, TR, TPR, EPT, V, FULL>;
@@ -199,12 +203,23 @@ __global__ void __launch_bounds__(norm_bwd_warps(TPR) * 32) norm_bwd_kernel(Norm
     }
 }
 
-// CTAs: as many as registers let stay resident, and no more partial sums than that
+// threads and elements of each for a row of D; with five sums per element a warp has no registers for eight elements and a second CTA
+struct NormBwdForm {
+    int tpr, ept;
+};
+static NormBwdForm norm_bwd_form(int D, bool full) {
+    if (D <= 256) return full ? NormBwdForm{64, 4} : NormBwdForm{32, 8};
+    if (D <= 512) return {64, 8};
+    if (D <= 1024) return {128, 8};
+    if (D <= 2048) return {256, 8};
+    return D <= 4096 ? NormBwdForm{256, 16} : NormBwdForm{512, 16};
+}
+// CTAs: those that stay resident, and no more partial sums than that
 static int norm_bwd_ctas(long long rows, int D, bool full) {
     const long long sms = sm_count() > 0 ? sm_count() : 148;
-    const long long per_sm = D <= 256 ? (full ? 1 : 2) : D <= 512 ? (full ? 6 : 12) : D <= 1024 ? (full ? 3 : 6) : D <= 2048 ? (full ? 1 : 3) : 1;
-    const long long most = D <= 256 ? ceil_div(rows, 8) : rows;
-    return (int)(most < sms * per_sm ? most : sms * per_sm);
+    const NormBwdForm f = norm_bwd_form(D, full);
+    const long long resident = sms * norm_bwd_resident(f.tpr, f.ept, full), most = f.tpr == 32 ? ceil_div(rows, 8) : rows;
+    return (int)(most < resident ? most : resident);
 }
 
 template <typename T, typename TR, int TPR, int EPT, bool FULL>
@@ -216,12 +231,16 @@ static int norm_bwd_launch(const NormParams& p, bool vec, int ctas, cudaStream_t
 }
 template <typename T, typename TR, bool FULL>
 static int norm_bwd_dispatch(const NormParams& p, bool vec, int ctas, cudaStream_t st) {
-    if (p.D <= 256) return norm_bwd_launch<T, TR, 32, 8, FULL>(p, vec, ctas, st);
-    if (p.D <= 512) return norm_bwd_launch<T, TR, 64, 8, FULL>(p, vec, ctas, st);
-    if (p.D <= 1024) return norm_bwd_launch<T, TR, 128, 8, FULL>(p, vec, ctas, st);
-    if (p.D <= 2048) return norm_bwd_launch<T, TR, 256, 8, FULL>(p, vec, ctas, st);
-    if (p.D <= 4096) return norm_bwd_launch<T, TR, 512, 8, FULL>(p, vec, ctas, st);
-    return norm_bwd_launch<T, TR, 1024, 8, FULL>(p, vec, ctas, st);
+    switch (norm_bwd_form(p.D, FULL).tpr) {
+        case 32: if constexpr (!FULL) return norm_bwd_launch<T, TR, 32, 8, FULL>(p, vec, ctas, st); break;
+        case 64: if (p.D > 256) return norm_bwd_launch<T, TR, 64, 8, FULL>(p, vec, ctas, st);
+                 if constexpr (FULL) return norm_bwd_launch<T, TR, 64, 4, FULL>(p, vec, ctas, st);
+                 break;
+        case 128: return norm_bwd_launch<T, TR, 128, 8, FULL>(p, vec, ctas, st);
+        case 256: return p.D > 2048 ? norm_bwd_launch<T, TR, 256, 16, FULL>(p, vec, ctas, st) : norm_bwd_launch<T, TR, 256, 8, FULL>(p, vec, ctas, st);
+        case 512: return norm_bwd_launch<T, TR, 512, 16, FULL>(p, vec, ctas, st);
+    }
+    return FWP_ERR_UNSUPPORTED;
 }
 
 }  // namespace fwp
