@@ -23,7 +23,7 @@ struct ConvParams {
     const float *w, *b;
     const int* lengths;
     float* part;                        // backward: [N * span groups][D * (K + 1)]
-    int N, L, D, silu, span, spans, groups;     // groups: of 32 x V channels
+    int N, L, D, silu, span, spans;
 };
 
 // V neighbouring channels of a step: one float, or two pairs for the two-wide instructions
@@ -377,7 +377,7 @@ FWP_API int fwp_causal_conv_forward(int N, int L, int D, int K, const fwp_tensor
     if ((rc = check_tensor(out, io_dtype == FWP_F32 ? 4 : 2, true))) return rc;
     DeviceGuard guard(device);
     if (guard.status) return guard.status;
-    ConvParams p = {stream_of(x), stream_of(state), stream_of(out), {}, {}, weight, bias, lengths, nullptr, N, L, D, silu ? 1 : 0, 0, 0, 0};
+    ConvParams p = {stream_of(x), stream_of(state), stream_of(out), {}, {}, weight, bias, lengths, nullptr, N, L, D, silu ? 1 : 0, 0, 0};
     return conv_dispatch(K, p, false, io_dtype, (cudaStream_t)stream);
 }
 
@@ -406,7 +406,7 @@ FWP_API int fwp_causal_conv_backward(int N, int L, int D, int K, const fwp_tenso
     }
     if (!scratch || !aligned16(scratch) || scratch_floats < fwp_causal_conv_backward_scratch_floats(N, L, D, K)) return FWP_ERR_SCRATCH;
     ConvParams p = {stream_of(x), stream_of(start), {}, stream_of(grad_out), stream_of(grad_x), weight, bias, lengths, scratch,
-                    N, L, D, silu ? 1 : 0, 0, 0, 0};
+                    N, L, D, silu ? 1 : 0, 0, 0};
     if ((rc = conv_dispatch(K, p, true, io_dtype, st))) return rc;
     const int V = conv_vectors(p, esz) ? 4 : 1;
     const int span = conv_span(N, L, D, V);
