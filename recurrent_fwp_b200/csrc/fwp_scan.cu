@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, PASS == SCAN_WHOLE ? 4 : 3) s
                 for (int c = 0; c < 2; c++) {
                     const float dl = c ? s.z : s.x, dx = c ? s.w : s.y;
                     const f2 d2 = f2_pack(dl, dl), x2 = f2_pack(dx, dx);
-                    const f2 e0 = exp2_pair(fmul2(d2, A[c][0])), e1 = exp2_pair(fmul2(d2, A[c][1]));
+                    const f2 e0 = decay_pair(d2, A[c][0]), e1 = decay_pair(d2, A[c][1]);
                     h[c][0] = ffma2(e0, h[c][0], fmul2(x2, b.x));
                     h[c][1] = ffma2(e1, h[c][1], fmul2(x2, b.y));
                     if (RAGGED) keep_states(h[c], 4 * j, p.S);
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(256) scan_join_kernel(ScanJoinParams q) {
             const bool on = k0 + i < p.spans - 1;
             const long long k = from + by * (k0 + i);
             end[i] = on ? ends[k * per_seq] : 0.f;
-            f[i] = on ? ex2_approx(dsum[k * p.D] * a) : 1.f;
+            f[i] = on ? decay_of(dsum[k * p.D], a) : 1.f;
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) {
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(128) scan_step_kernel(ScanParams p) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
             if (4 * j + i < p.S) {
-                h[q][i] = fmaf(ex2_approx(e * a[i]), h[q][i], ex * (VEC ? B[q][0].get(i) : B[q][VEC ? 0 : i].get(0)));
+                h[q][i] = fmaf(decay_of(e, a[i]), h[q][i], ex * (VEC ? B[q][0].get(i) : B[q][VEC ? 0 : i].get(0)));
                 y[q] = fmaf(VEC ? C[q][0].get(i) : C[q][VEC ? 0 : i].get(0), h[q][i], y[q]);
             }
         if (!live[q] || !on || !p.state) continue;

@@ -86,9 +86,14 @@ __device__ __forceinline__ float softplus_(float x) {
     return fmaf(2.f * s, r, fmaxf(x, 0.f));     // a NaN is in s
 }
 
-__device__ __forceinline__ f2 exp2_pair(f2 v) {
+// exp(delta A) from A log2(e).  A slow channel multiplies a thousand of these, so it is the mean error of the exponential instruction that
+// its state shows: measured -19e-9 (relative) for arguments between -0.1 and -0.002, -5e-9 below.  2^-26 on the argument, which rides on the
+// product for free, makes that -9e-9 and +5e-9; zero still gives exactly one.  The gradient of A over 2048 steps: 1.6e-6 -> 0.7e-6 off.
+constexpr float kDecayCentre = 1.f / 67108864.f;
+__device__ __forceinline__ float decay_of(float delta, float a) { return ex2_approx(fmaf(delta, a, kDecayCentre)); }
+__device__ __forceinline__ f2 decay_pair(f2 delta, f2 a) {
     float lo, hi;
-    f2_unpack(v, lo, hi);
+    f2_unpack(ffma2(delta, a, f2_pack(kDecayCentre, kDecayCentre)), lo, hi);
     return f2_pack(ex2_approx(lo), ex2_approx(hi));
 }
 
