@@ -205,6 +205,9 @@ struct ScanJoinParams {
     ScanParams p;
     int backwards;
 };
+// exp(A sum delta) h from the root of the factor.  Where states grow the factor of a span may pass the range of a float though no step's does and
+// its product with h does not either, so it is taken in two halves; a zero stays zero and an infinity stays one, as step after step leaves them.
+__device__ __forceinline__ float over_span(float h, float root) { return h == 0.f || isinf(h) ? h : h * root * root; }
 __global__ void __launch_bounds__(256) scan_join_kernel(ScanJoinParams q) {
     const ScanParams& p = q.p;
     griddep_wait();
@@ -223,12 +226,12 @@ __global__ void __launch_bounds__(256) scan_join_kernel(ScanJoinParams q) {
             const bool on = k0 + i < p.spans - 1;
             const long long k = from + by * (k0 + i);
             end[i] = on ? ends[k * per_seq] : 0.f;
-            f[i] = on ? decay_of(dsum[k * p.D], a) : 1.f;
+            f[i] = on ? decay_of(0.5f * dsum[k * p.D], a) : 1.f;
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             if (k0 + i < p.spans) ends[(from + by * (k0 + i)) * per_seq] = h;
-            h = fmaf(f[i], h, end[i]);
+            h = over_span(h, f[i]) + end[i];
         }
     }
 }
