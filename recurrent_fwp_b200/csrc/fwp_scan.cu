@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, PASS == SCAN_WHOLE ? 4 : 3) s
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int st = 4 * j + i;
-            a[i] = st < p.S ? p.A[(long long)d[c] * p.S + st] * kLog2e : 0.f;
+            a[i] = st < p.S ? rate_of(p.A[(long long)d[c] * p.S + st]) : 0.f;
             s[i] = 0.f;
             if (WHOLE && st < p.S) {
                 if (p.spans > 1) s[i] = p.ends[(spans_at + d[c]) * p.S + st];
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(256) scan_join_kernel(ScanJoinParams q) {
     const long long e = (long long)blockIdx.x * 256 + threadIdx.x, per_seq = (long long)p.D * p.S;
     if (e >= per_seq) return;
     const int n = blockIdx.y, d = (int)(e / p.S), s = (int)(e - (long long)d * p.S);
-    const float a = p.A[e] * kLog2e;
+    const float a = rate_of(p.A[e]);
     float h = !q.backwards && p.state ? p.state[n * p.state_sN + d * p.state_sD + s] : 0.f;
     float* ends = p.ends + (long long)n * p.spans * per_seq + e;
     const float* dsum = p.dsums + (long long)n * p.spans * p.D + d;
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(128) scan_step_kernel(ScanParams p) {
     }
     float a[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) a[i] = 4 * j + i < p.S ? p.A[(long long)d * p.S + 4 * j + i] * kLog2e : 0.f;
+    for (int i = 0; i < 4; i++) a[i] = 4 * j + i < p.S ? rate_of(p.A[(long long)d * p.S + 4 * j + i]) : 0.f;
     const float bias = p.dt_bias ? p.dt_bias[d] : 0.f, skip = p.skip ? p.skip[d] : 0.f;
     float y[kStepSeqs];
 #pragma unroll

@@ -1,5 +1,6 @@
 // Parameters and device pieces of the selective scan, shared by its forward (fwp_scan.cu) and backward (fwp_scan_bwd.cu).
 #pragma once
+#include <cfloat>
 #include "fwp_seq.cuh"
 
 namespace fwp {
@@ -84,6 +85,13 @@ __device__ __forceinline__ float softplus_(float x) {
     r = fmaf(r, q, 1.f / 3.f);
     r = fmaf(r, q, 1.f);
     return fmaf(2.f * s, r, fmaxf(x, 0.f));     // a NaN is in s
+}
+
+// A log2(e).  Minus infinity, a state that keeps nothing, counts as the most negative float: steps of size zero, those behind the end of a
+// sequence among them, leave such a state alone too, where zero times infinity would be NaN.
+__device__ __forceinline__ float rate_of(float a) {
+    a *= kLog2e;
+    return a < -FLT_MAX ? -FLT_MAX : a;
 }
 
 // exp(delta A) from A log2(e).  A slow channel multiplies a thousand of these, so it is the mean error of the exponential instruction that

@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kBwdWarps * 32, 2) scan_bwd_kernel(ScanParams 
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const bool in = 4 * j + i < p.S;
-            a[i] = in ? p.A[(long long)d[c] * p.S + 4 * j + i] * kLog2e : 0.f;
+            a[i] = in ? rate_of(p.A[(long long)d[c] * p.S + 4 * j + i]) : 0.f;
             s[i] = in && WHOLE && p.spans > 1 ? p.ends[(spans_at + d[c]) * p.S + 4 * j + i] : 0.f;
         }
         A[c][0] = f2_pack(a[0], a[1]); A[c][1] = f2_pack(a[2], a[3]);

@@ -9,6 +9,7 @@
     float32 or bfloat16, and take any outer strides (slices of a projection as they are).  ``A`` (D, S) with S <= 64, ``D`` (D,)
     and ``dt_bias`` (D,) are float32.  ``D``, ``z`` and ``dt_bias`` may be left out; ``softplus=False`` takes dt + dt_bias as it is.
     A may have either sign: states that grow (A > 0, or negative step sizes) are as far from the definition as float32 steps leave them.
+    Minus infinity is a state that keeps nothing.
   * ``state`` (N, D, S) float32 enters as the state before the first step and is overwritten with the state after the last, so that
     segments, and single tokens (L = 1), follow on from one another.  Without it the scan starts from zeros.  As with the fast weight
     ops no gradient flows to it; unlike theirs, ``backward`` does not rewind it (a state that decays cannot be run backwards).

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from oracle import blocks
 from recurrent_fwp_b200 import _lib
 from tests import util
 from tests.blocks_util import DEV, close
@@ -61,3 +62,23 @@ def test_infinite_states_stay_infinite(fwp, chunk):
     assert torch.isinf(state[1, 7, 3])
     state[1, 7, 3] = 0
     assert torch.isfinite(state).all()
+
+
+@pytest.mark.parametrize('lengths', [None, 'inside'])
+@pytest.mark.parametrize('L', [1, 12, 300])
+def test_states_that_keep_nothing(fwp, chunk, L, lengths):
+    """A of minus infinity: the state is the last step's input alone, and steps behind the end leave it.  In the definition -1e30 stands for it:
+    its gradient of the step size would be zero times infinity."""
+    a, gy = make(4, 3, L, 24, 16, lengths=lengths)
+    a['A'][::3, 5] = -1e30
+    b = dict(a, A=torch.where(a['A'] < -1e29, -float('inf'), a['A']))
+    ref, end, sums = blocks.selective_scan(**a, gy=gy)
+    out, state, grads = run(fwp, b, gy)
+    close('out', out, ref, steps=L)
+    close('state', state, end, steps=L)
+    for k, g in grads.items():
+        close('gradient of ' + k, g, *sums[k], steps=L)
+    state = a['state'].clone()
+    with torch.no_grad():
+        close('out', fwp.selective_scan(**dict(b, state=state)), ref, steps=L)
+    close('state', state, end, steps=L)
