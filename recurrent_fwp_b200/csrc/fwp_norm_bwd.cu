@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(norm_bwd_warps(TPR) * 32, norm_bwd_resident(TP
         f2 t[FULL ? P : 1], a[FULL ? P : 1], da[FULL ? P : 1], sc[FULL ? P : 1], w[P];
         if constexpr (FULL) {
             if (p.pw) {
-                const f2 s = f2_all(stats.y), m = f2_all(-stats.x * stats.y);
+                const f2 s = f2_all(stats.y), m = f2_all(-stats.x);
                 row_load<TPR, EPT, V>(p.pw, p.D, tid, w);
                 if (p.pb) row_load<TPR, EPT, V>(p.pb, p.D, tid, t);
                 else
@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(norm_bwd_warps(TPR) * 32, norm_bwd_resident(TP
                     for (int i = 0; i < P; i++) t[i] = 0;
 #pragma unroll
                 for (int i = 0; i < P; i++) {
-                    x[i] = ffma2(x[i], s, m);
+                    x[i] = fmul2(fadd2(x[i], m), s);        // in the forward's order: rows may be large against their spread, or constant
                     t[i] = ffma2(x[i], w[i], t[i]);         // zero beyond the row, where w and b are
                 }
             } else {
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(norm_bwd_warps(TPR) * 32, norm_bwd_resident(TP
             for (int i = 0; i < P; i++) r[i] = ffma2(s, x[i], r[i]);
         }
         row_load<TPR, EPT, V>(p.w, p.D, tid, w);
-        // the mean is taken off before the scaling, as in the forward: r may be large against its spread
+        // here too the mean is taken off before the scaling
         const f2 rs = f2_all(stats.w), mean = f2_all(-stats.z);
         f2 s0 = 0, s1 = 0;
 #pragma unroll
