@@ -7,7 +7,8 @@ and the norm before the next block.
     r = residual + scale u                              y = norm(r) weight + bias
 
   * ``x``, the output of a block, and ``gate`` (..., D) share one type, float32 or bfloat16; ``y`` has it too.  ``residual`` has that
-    type or float32, and ``r``, the new residual, has the residual's.  Rows may have any outer strides, D <= 8192.
+    type or float32, and ``r``, the new residual, has the residual's.  Rows may have any outer strides, D <= 8192; with more than
+    three dimensions, streams whose outer dimensions do not merge into one are copied first.
   * ``weight``, ``bias``, ``post_weight``, ``post_bias`` (D,) are float32; ``scale`` is a float32 (D,) tensor or a number.
   * ``gate_act``: 'silu', 'sigmoid' or 'identity'.  ``rms=True``: root-mean-square norms (no mean is taken off) instead of LayerNorms.
   * everything but x and weight may be left out; without a residual r is scale u.
@@ -54,7 +55,7 @@ def block_norm(x, weight, bias=None, residual=None, scale=None, gate=None, post_
         raise ValueError("gate_act is 'silu', 'sigmoid' or 'identity', got %r" % (gate_act,))
     if x.dim() > 3:
         shape = x.shape
-        x, residual, gate = (None if t is None else t.reshape(-1, t.shape[-1]) if t.shape == shape else t for t in (x, residual, gate))
+        x, residual, gate = (None if t is None else t.flatten(0, -2) if t.shape == shape else t for t in (x, residual, gate))
         y, r = _block_norm(x, weight, bias, residual, scale, gate, post_weight, post_bias, _ACTS[gate_act], eps, rms)
         return y.view(shape), r.view(shape)
     return _block_norm(x, weight, bias, residual, scale, gate, post_weight, post_bias, _ACTS[gate_act], eps, rms)

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from oracle import blocks
-from tests.blocks_util import close
+from tests.blocks_util import DEV, close
 from tests.test_block_norm_gpu import make, run, sizes
 
 pytestmark = pytest.mark.gpu
@@ -24,3 +24,13 @@ def test_constant_rows_with_a_norm_behind_the_block(fwp, D, types):
     sums = blocks.block_norm(**a, gy=gy, gr=gr)[2]
     for k, g in grads.items():
         close('gradient of ' + k, g, sums[k][0], sizes(*sums[k], D))
+
+
+@pytest.mark.parametrize('shape', [(2, 0), (2, 3, 0), (2, 3, 4, 0), (2, 0, 4, 8)])
+def test_rows_without_elements(fwp, shape):
+    x, res, gate = (torch.zeros(shape, device=DEV).requires_grad_() for _ in range(3))
+    w = torch.ones(shape[-1], device=DEV).requires_grad_()
+    y, r = fwp.block_norm(x, w, residual=res, gate=gate)
+    assert y.shape == r.shape == shape
+    grads = torch.autograd.grad([y, r], [x, w, res, gate], [torch.ones_like(y), torch.ones_like(r)])
+    assert [g.shape for g in grads] == [t.shape for t in (x, w, res, gate)] and not any(g.any() for g in grads)
