@@ -335,14 +335,23 @@ static ScanPlan scan_plan(int N, int L, int D, int S, int G) {
     if (forced > 0) spans = ceil_div(L, ceil_div(forced, tile) * tile);
     else if (ctas * 3 <= sms * 2) {
         spans = sms * 2 / ctas;
-        const long long most = ceil_div(L, 2 * tile);
+        const long long most = ceil_div(L, L <= 512 ? tile : 2 * tile);        // the join goes through them one by one: 1 x 4096 x 64, spans of 32 and 64: 53 and 37 us
         if (spans > most) spans = most;
     }
     if (spans > 4096) spans = 4096;
-    ScanPlan q;
-    q.span = (int)(ceil_div(ceil_div(L, spans), tile) * tile);
-    q.spans = (int)ceil_div(L, q.span);
-    return q;
+    auto cut = [&](long long n) {
+        ScanPlan q;
+        q.span = (int)(ceil_div(ceil_div(L, n), tile) * tile);
+        q.spans = (int)ceil_div(L, q.span);
+        return q;
+    };
+    const ScanPlan q = cut(spans);
+    if (forced > 0 || q.spans == 1) return q;
+    // And they have to shorten the chain: a span is walked twice, 1.23 times as long a step where SMs have two CTAs, and the two launches beside the
+    // first take about 48 steps' time.  One launch against spans (bf16, 16 states, 2048 channels): one sequence of 96 steps 11.8 and 12.0 us, 112 steps
+    // 13.4 and 12.6, 256 steps 27.8 and 16.1; two of 160 steps 18.1 and 19.7, 192 steps 21.4 and 19.9; three of 320 steps 34.4 and 37.7, 384 steps 40.8 and 38.4.
+    const long long walked = 2LL * q.span, beside = ctas * q.spans > sms ? ctas * q.spans - sms : 0;
+    return walked + walked * beside * 23 / (sms * 100) + 48 > L ? cut(1) : q;
 }
 
 template <typename T, int LPC, bool RAGGED, bool PAIRS>
