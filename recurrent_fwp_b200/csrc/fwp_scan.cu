@@ -338,7 +338,7 @@ static ScanPlan scan_plan(int N, int L, int D, int S, int G) {
         const long long most = ceil_div(L, L <= 512 ? tile : 2 * tile);        // the join goes through them one by one: 1 x 4096 x 64, spans of 32 and 64: 53 and 37 us
         if (spans > most) spans = most;
     }
-    if (spans > 4096) spans = 4096;
+    if (spans > 2048) spans = 2048;         // rounded up to the tile they end within 2^16 of the sequence: see kMaxSteps
     auto cut = [&](long long n) {
         ScanPlan q;
         q.span = (int)(ceil_div(ceil_div(L, n), tile) * tile);

@@ -32,3 +32,15 @@ def test_spans_are_taken_where_they_shorten_the_chain(shape):
         taken.append(n)
     many = N * -(-D // (256 // max(1, -(-S // 4)))) * 3 > 148 * 2       # CTAs, of 64 channels at 16 states
     assert (max(taken) == 1) == many
+
+
+def test_the_last_step_of_the_last_span_is_an_int():
+    """Spans asked for by ``scan.chunk`` are rounded up to 32 steps each; behind the longest sequence all of them end below 2^31."""
+    longest = 0x7fff0000
+    try:
+        _lib.tune('scan.chunk', 32)
+        n = spans_of(1, longest, 1, 1)
+    finally:
+        _lib.tune('scan.chunk', 0)
+    span = -(-(-(-longest // n)) // 32) * 32
+    assert n * span < 2 ** 31
