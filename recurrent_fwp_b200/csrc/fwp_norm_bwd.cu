@@ -15,13 +15,17 @@ constexpr int norm_bwd_resident(int TPR, int EPT, bool FULL) {
     return TPR == 32 ? 2 : EPT == 4 || (EPT == 8 && !FULL) ? 24 / norm_bwd_warps(TPR) : EPT == 8 || !FULL ? 16 / norm_bwd_warps(TPR) : 1;
 }
 
-// Rows ahead of the one at work: two where shared memory has room
+// Rows ahead of the one at work: two where shared memory has room for all the CTAs that an SM is to hold.  fp32 rows of 2049 to 4096 with the
+// residual sum alone have room for two CTAs with one row ahead or one CTA with two: 107 and 112 us for 32 Mi elements at 4096, 153 and 180 us at 2052.
 template <typename T, typename TR, int TPR, int EPT, int V, bool FULL>
 struct NormBwdRing {
     static constexpr int SLOTS = TPR == 32 ? 8 : 1, ROW = TPR * EPT;
     static constexpr int kGy = ROW * sizeof(T), kGate = 2 * kGy, kRes = (FULL ? 3 : 2) * kGy, kGr = kRes + ROW * sizeof(TR), kStage = kGr + ROW * sizeof(TR);
     static constexpr int kRed = SLOTS > 1 ? SLOTS * ROW * 4 : 0;
-    static constexpr int DEPTH = V != 4 ? 0 : 2 * SLOTS * kStage + kRed <= 230000 ? 2 : 1;
+    // of an SM's 227 KB, less 1 KB that every CTA takes for itself
+    static constexpr int kRoom = (227 * 1024) / norm_bwd_resident(TPR, EPT, FULL) - 1024 - 4 * 8 * (TPR / 32);
+    static constexpr int DEPTH = V != 4 ? 0 : 2 * SLOTS * kStage + kRed <= kRoom ? 2 : 1;
+    static_assert(V != 4 || SLOTS * DEPTH * kStage + kRed <= kRoom, "the CTAs that an SM is to hold do not fit");
     static constexpr size_t bytes = (size_t)SLOTS * DEPTH * kStage + kRed;
 };
 
