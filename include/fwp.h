@@ -403,7 +403,8 @@ int fwp_fast_lstm_backward_from_outputs(int variant, int N, int H, int L, int D,
  * outputs and gradients are zero; values are taken between 0 and L.  N, L, D may be 0: nothing is read or written then.
  * States are fp32, in/out in the forwards.  The backwards neither read nor rewind them: a state that decays cannot be run
  * backwards, so they start from what the forward kept (`start`, `checkpoints`).  No gradient reaches a state.
- * Scratch and checkpoints are the caller's, 16-byte aligned, contents undefined before.
+ * Scratch and checkpoints are the caller's, 16-byte aligned, contents undefined before.  Their sizes may depend on the number of SMs: those asked
+ * for without a device do on every device of the machine.
  *
  * Short causal convolution per channel, K taps (1 <= K <= 8):
  *   p_t = bias + sum_j weight[d, j] x_{t-K+1+j},  out_t = silu ? p_t sigmoid(p_t) : p_t

@@ -49,6 +49,22 @@ int sm_count() {
     return n;
 }
 
+int most_sms() {
+    static std::atomic<int> cached{0};
+    int most = cached.load(std::memory_order_relaxed);
+    if (most) return most;
+    int devices = 0;
+    if (cudaGetDeviceCount(&devices) != cudaSuccess) return 148;
+    for (int d = 0; d < devices; d++) {
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, d) != cudaSuccess) return 148;
+        if (n > most) most = n;
+    }
+    if (!most) return 148;
+    cached.store(most, std::memory_order_relaxed);
+    return most;
+}
+
 int tune_get(TuneKey key, int fallback) {
     const int v = g_tune.v[key].load(std::memory_order_relaxed);
     return v == INT_MIN ? fallback : v;

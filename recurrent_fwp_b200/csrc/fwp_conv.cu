@@ -265,9 +265,10 @@ __global__ void __launch_bounds__(kConvWarps * 32, K > 4 ? 2 : sizeof(T) == 2 ? 
     }
 }
 
+static long long conv_sms() { return sm_count() > 0 ? sm_count() : 148; }
 // Steps a warp walks: long spans read fewer neighbours' steps, short ones fill the machine when there are few channels.
-static int conv_span(int N, int L, int D, int V) {
-    const long long columns = (long long)N * ceil_div(D, 32 * V), sms = sm_count() > 0 ? sm_count() : 148;
+static int conv_span(int N, int L, int D, int V, long long sms) {
+    const long long columns = (long long)N * ceil_div(D, 32 * V);
     int span = 64;
     while (span > kConvSpan && columns * ceil_div(L, span) < sms * 16) span >>= 1;
     while (ceil_div(L, (long long)span * kConvWarps) > 65535) span <<= 1;      // the grid's limit
@@ -294,7 +295,7 @@ static bool conv_vectors(const ConvParams& p, int esz) {
 
 template <typename T, int K, int V>
 static int conv_launch(ConvParams p, bool backward, cudaStream_t st) {
-    p.span = conv_span(p.N, p.L, p.D, V);
+    p.span = conv_span(p.N, p.L, p.D, V, conv_sms());
     p.spans = (int)ceil_div(p.L, p.span);
     const dim3 grid((unsigned)ceil_div(p.D, 32 * V), (unsigned)ceil_div(p.spans, kConvWarps), (unsigned)p.N);
     if (backward) return launch_dependent(conv_bwd_kernel<T, K, V>, p, grid, kConvWarps * 32, 0, st, "conv_bwd_kernel");
@@ -319,10 +320,10 @@ static int conv_dispatch(int K, const ConvParams& p, bool backward, int io_dtype
 }
 
 // rows of partial sums: at most those of the narrowest form
-static long long conv_part_rows(int N, int L, int D) {
+static long long conv_part_rows(int N, int L, int D, long long sms) {
     long long most = 0;
     for (int V : {1, 4}) {
-        int span = conv_span(N, L, D, V);
+        int span = conv_span(N, L, D, V, sms);
         const long long rows = (long long)N * ceil_div(ceil_div(L, span), kConvWarps);
         most = rows > most ? rows : most;
     }
@@ -383,7 +384,7 @@ FWP_API int fwp_causal_conv_forward(int N, int L, int D, int K, const fwp_tensor
 
 FWP_API int64_t fwp_causal_conv_backward_scratch_floats(int N, int L, int D, int K) {
     if (N <= 0 || L <= 0 || D <= 0 || K < 1 || K > kConvMaxK) return 0;
-    return conv_part_rows(N, L, D) * D * (K + 1);
+    return conv_part_rows(N, L, D, most_sms()) * D * (K + 1);        // more SMs never take fewer rows
 }
 
 FWP_API int fwp_causal_conv_backward(int N, int L, int D, int K, const fwp_tensor* x, const float* weight, const float* bias,
@@ -404,12 +405,12 @@ FWP_API int fwp_causal_conv_backward(int N, int L, int D, int K, const fwp_tenso
         if (e == cudaSuccess && D && grad_bias) e = cudaMemsetAsync(grad_bias, 0, sizeof(float) * D, st);
         return e == cudaSuccess ? FWP_OK : set_cuda_error(e);
     }
-    if (!scratch || !aligned16(scratch) || scratch_floats < fwp_causal_conv_backward_scratch_floats(N, L, D, K)) return FWP_ERR_SCRATCH;
+    if (!scratch || !aligned16(scratch) || scratch_floats < conv_part_rows(N, L, D, conv_sms()) * D * (K + 1)) return FWP_ERR_SCRATCH;
     ConvParams p = {stream_of(x), stream_of(start), {}, stream_of(grad_out), stream_of(grad_x), weight, bias, lengths, scratch,
                     N, L, D, silu ? 1 : 0, 0, 0};
     if ((rc = conv_dispatch(K, p, true, io_dtype, st))) return rc;
     const int V = conv_vectors(p, esz) ? 4 : 1;
-    const int span = conv_span(N, L, D, V);
+    const int span = conv_span(N, L, D, V, conv_sms());
     const long long dk = (long long)D * K;
     ColumnSums s = {scratch, (int)(N * ceil_div(ceil_div(L, span), kConvWarps)), dk + D, {grad_weight, grad_bias}, {dk, dk + D}};
     return launch_column_sums(s, st);

@@ -74,6 +74,7 @@ enum TuneKey {
 };
 int tune_get(TuneKey key, int fallback);
 int sm_count();             // SMs of the current device
+int most_sms();             // SMs of the machine's largest device, 148 where none can be asked: for workspaces that have to do on every one
 
 // Sequences per CTA: a divisor of the sequence count, and fewer while that lowers the number an SM gets at most -- with
 // few sequences the warps of one are better spread over the four schedulers of an SM of their own (d = 32, 512 steps, 32

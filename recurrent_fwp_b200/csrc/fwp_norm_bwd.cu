@@ -219,11 +219,15 @@ static NormBwdForm norm_bwd_form(int D, bool full) {
     return D <= 4096 ? NormBwdForm{256, 16} : NormBwdForm{512, 16};
 }
 // CTAs: those that stay resident, and no more partial sums than that
-static int norm_bwd_ctas(long long rows, int D, bool full) {
-    const long long sms = sm_count() > 0 ? sm_count() : 148;
+static int norm_bwd_ctas(long long rows, int D, bool full, long long sms) {
     const NormBwdForm f = norm_bwd_form(D, full);
     const long long resident = sms * norm_bwd_resident(f.tpr, f.ept, full), most = f.tpr == 32 ? ceil_div(rows, 8) : rows;
     return (int)(most < resident ? most : resident);
+}
+
+static int64_t norm_bwd_scratch(long long rows, int D, long long sms) {
+    const int a = norm_bwd_ctas(rows, D, true, sms), b = norm_bwd_ctas(rows, D, false, sms);
+    return (int64_t)(a > b ? a : b) * D * 5;
 }
 
 template <typename T, typename TR, int TPR, int EPT, bool FULL>
@@ -253,8 +257,7 @@ using namespace fwp;
 
 FWP_API int64_t fwp_block_norm_backward_scratch_floats(int N, int L, int D) {
     if (N <= 0 || L <= 0 || D <= 0 || D > kNormMaxD) return 0;
-    const long long rows = (long long)N * L;
-    return (int64_t)(norm_bwd_ctas(rows, D, true) > norm_bwd_ctas(rows, D, false) ? norm_bwd_ctas(rows, D, true) : norm_bwd_ctas(rows, D, false)) * D * 5;
+    return norm_bwd_scratch((long long)N * L, D, most_sms());
 }
 
 FWP_API int fwp_block_norm_backward(int N, int L, int D, const fwp_tensor* x, const fwp_tensor* residual, const fwp_tensor* gate,
@@ -285,7 +288,8 @@ FWP_API int fwp_block_norm_backward(int N, int L, int D, const fwp_tensor* x, co
     }
     if (!stats) return FWP_ERR_NULL;
     if (!aligned16(stats)) return FWP_ERR_ALIGN;
-    if (!scratch || !aligned16(scratch) || scratch_floats < fwp_block_norm_backward_scratch_floats(N, L, D)) return FWP_ERR_SCRATCH;
+    const long long sms = sm_count() > 0 ? sm_count() : 148;
+    if (!scratch || !aligned16(scratch) || scratch_floats < norm_bwd_scratch((long long)N * L, D, sms)) return FWP_ERR_SCRATCH;
     NormParams p = norm_params(N, L, D, x, residual, gate, scale_vector, scale_value, post_weight, post_bias, weight, bias, rms, gate_act);
     p.gy = stream_of(grad_y); p.gr = stream_of(grad_r); p.gx = stream_of(grad_x); p.gres = stream_of(grad_residual);
     p.ggate = stream_of(grad_gate);
@@ -295,7 +299,7 @@ FWP_API int fwp_block_norm_backward(int N, int L, int D, const fwp_tensor* x, co
     for (const Stream* s : {&p.x, &p.gate, &p.gy, &p.gx, &p.ggate}) vec = vec && rows_aligned(*s, esz, 4 * esz);
     for (const Stream* s : {&p.res, &p.gr, &p.gres}) vec = vec && rows_aligned(*s, rsz, 4 * rsz);
     const bool full = p.pw || p.gate.p || p.sv;
-    const int ctas = norm_bwd_ctas(p.rows, D, full);
+    const int ctas = norm_bwd_ctas(p.rows, D, full, sms);
     auto run = [&](auto t, auto r) {
         using T = decltype(t);
         using TR = decltype(r);
