@@ -82,3 +82,72 @@ def test_states_that_keep_nothing(fwp, chunk, L, lengths):
     with torch.no_grad():
         close('out', fwp.selective_scan(**dict(b, state=state)), ref, steps=L)
     close('state', state, end, steps=L)
+
+
+def rel(a, b):
+    return ((a.double() - b).norm() / b.norm()).item()
+
+
+@pytest.mark.parametrize('band', [(0.002, 0.1), (0.0001, 0.002)])
+def test_the_mean_error_of_a_decay(fwp, band):
+    """A slow channel multiplies a thousand decays, so their mean error is what its state shows: -9e-9 for arguments of the base-2 exponential
+    between -0.1 and -0.002, +5e-9 towards zero (the instruction by itself: -19e-9 and -5e-9).  65536 states of 64 steps: the mean's own
+    deviation is below 1e-10 (a step rounds to within 6e-8), so 12e-9 tells them apart and holds both."""
+    L, M, S = 64, 4096, 16
+    g = util.gen(5)
+    lo, hi = (torch.tensor(b).log() for b in band)
+    A = -torch.exp(lo + torch.rand(M, S, generator=g) * (hi - lo)).to(DEV) * 0.6931471805599453
+    dt = (1 + 0.1 * torch.randn(1, L, M, generator=g)).to(DEV)
+    state, zero = torch.ones(1, M, S, device=DEV), torch.zeros(1, L, M, device=DEV)
+    _lib.tune('scan.chunk', 1 << 20)
+    try:
+        with torch.no_grad():
+            fwp.selective_scan(zero, dt, A, zero[..., :S], zero[..., :S], state=state, softplus=False)
+    finally:
+        _lib.tune('scan.chunk', 0)
+    ref = torch.exp(dt.double().sum(1)[..., None] * A.double())
+    assert abs((state.double() / ref - 1).mean().item() / L) <= 12e-9
+
+
+def test_long_sequences_to_the_accuracy_of_their_decays(fwp, chunk):
+    """2048 steps of channels that keep 10 to 500 of them.  A state that keeps T steps is off by T times the decays' mean error; its square
+    grows like T, so over T spread evenly on a logarithmic scale the 2-norm is off by 500 / sqrt(3) mean errors of 9e-9: 2.6e-6.  The
+    gradient of A is made of two such recurrences: twice that."""
+    g = util.gen(6)
+    r = lambda *s: torch.randn(*s, generator=g).to(DEV)         # noqa: E731
+    N, L, M, S = 1, 2048, 32, 16
+    rate = torch.exp(torch.rand(M, S, generator=g) * torch.tensor(50.).log()).to(DEV) * 0.002
+    a = dict(x=r(N, L, M), dt=0.1 * r(N, L, M), A=-rate / 0.05, B=r(N, L, S), C=r(N, L, S), D=r(M), z=r(N, L, M),
+             dt_bias=torch.full((M,), -2.97, device=DEV), state=r(N, M, S))      # softplus(-2.97) = 0.05
+    gy = r(N, L, M)
+    ref, end, sums = blocks.selective_scan(**a, gy=gy)
+    out, state, grads = run(fwp, a, gy)
+    most = 500 / 3 ** 0.5 * 9e-9
+    assert rel(out, ref) <= most and rel(state, end) <= most
+    for k, t in grads.items():
+        assert rel(t, sums[k][0]) <= (2 * most if k == 'A' else most), k
+
+
+def test_a_training_step_of_a_wide_layer(fwp):
+    """8 x 2048 steps of 2048 channels in bf16, step sizes over 0.001 ... 0.1 and rates 1 ... 16: a few channels, which are recurrences of
+    their own, against the definition.  bf16 results are off by half a step of 2^-8 each; the slowest channel keeps 1000 steps (see above)."""
+    g = util.gen(7)
+    N, L, M, S = 8, 2048, 2048, 16
+    cuda = torch.Generator(device=DEV)
+    cuda.manual_seed(7)
+    r = lambda *s: torch.randn(*s, generator=cuda, device=DEV).to(BF16)         # noqa: E731
+    step = torch.exp(torch.rand(M, generator=g) * torch.tensor(100.).log()).to(DEV) * 0.001
+    a = dict(x=r(N, L, M), dt=r(N, L, M), A=-torch.arange(1., S + 1, device=DEV).repeat(M, 1), B=r(N, L, S), C=r(N, L, S),
+             D=torch.ones(M, device=DEV), z=r(N, L, M), dt_bias=torch.log(torch.expm1(step)), state=r(N, M, S).float() * 0.1, lengths=None)
+    gy = r(N, L, M)
+    out, state, grads = run(fwp, a, gy)
+    some = torch.randperm(M, generator=g)[:12].to(DEV)
+    b = {k: a[k][..., some] if k in ('x', 'dt', 'z', 'dt_bias', 'D') else a[k] for k in a}
+    b.update(A=a['A'][some], state=a['state'][:, some])
+    ref, end, sums = blocks.selective_scan(**b, gy=gy[..., some])
+    slow = 1000 / 3 ** 0.5 * 9e-9
+    assert rel(out[..., some], ref) <= 2 ** -8 and rel(state[:, some], end) <= slow
+    for k in ('x', 'dt', 'z'):
+        assert rel(grads[k][..., some], sums[k][0]) <= 2 ** -8, k
+    for k in ('A', 'D', 'dt_bias'):
+        assert rel(grads[k][some], sums[k][0]) <= 2 * slow, k
