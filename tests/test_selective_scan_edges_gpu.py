@@ -151,3 +151,17 @@ def test_a_training_step_of_a_wide_layer(fwp):
         assert rel(grads[k][..., some], sums[k][0]) <= 2 ** -8, k
     for k in ('A', 'D', 'dt_bias'):
         assert rel(grads[k][some], sums[k][0]) <= 2 * slow, k
+
+
+def test_the_relative_error_of_small_step_sizes(fwp):
+    """softplus: 3e-7 + 7e-8 |x| relative, which comes from the product in the exponential's argument, down to -87; zero below -87.4."""
+    x = torch.cat([torch.linspace(-100, 30, 1 << 20), torch.linspace(-1, 1, 1 << 18)]).to(DEV)
+    M = 4096
+    state, one = torch.zeros(x.numel() // M, M, 1, device=DEV), torch.ones(x.numel() // M, 1, M, device=DEV)
+    with torch.no_grad():       # one step from zero with unit inputs leaves the step size itself
+        fwp.selective_scan(one, x.view(-1, 1, M), -torch.ones(M, 1, device=DEV), one[..., :1], one[..., :1], state=state)
+    got, x = state.flatten().double(), x.double()
+    ref = x.clamp(min=0) + torch.log1p(torch.exp(-x.abs()))
+    kept = x >= -87
+    assert (((got - ref) / ref).abs() <= 3e-7 + 7e-8 * x.abs())[kept].all()
+    assert not got[x < -87.4].any()
