@@ -8,8 +8,9 @@
 // lane with the value of one step; that lane loads x, dt, z for it and stores its output, so y goes through no memory.
 //
 // The exponentials bound it: S per (step, channel), 16 a clock and SM.  At 8 x 2048 x 2048 (bf16, S = 16) that is 115 us, and 29 us more for
-// softplus and silu; measured 290 us, 321 us with checkpoints.  With one channel per lane shared memory was the limit (B and C read for 8
-// channels at a time, 89 % of the pipe, 383 us); with two it is the latency of 1.7 warps per scheduler (exponential unit 48 %, issue 47 %).
+// softplus and silu; measured 293 us, 321 us with checkpoints.  With one channel per lane shared memory was the limit (B and C read for 8
+// channels at a time, 89 % of the pipe, 383 us); with two it is the latency of 1.7 warps per scheduler (exponential unit 48 %, issue 48 %,
+// shared memory 47 %; four CTAs of 128 registers would fit, there are 256 for 148 SMs).
 #include "fwp_scan.cuh"
 
 namespace fwp {

@@ -9,7 +9,7 @@
 // twice: twelve exponentials per state and tile where eight steps in registers would take eight, for two channels at a time, which
 // halves the reads of B and C and the shuffles below.  Sums over states end in the lane that loads and stores the (step, channel).  The
 // sums over channels, gB and gC, halve their way through the lanes of a warp, meet the CTA's other warps in shared memory and leave as one
-// row per CTA and step, added up in a fixed order by scan_bc_kernel: no atomics.  8 x 2048 x 2048 (bf16, S = 16): 879 us, 217 instructions per
+// row per CTA and step, added up in a fixed order by scan_bc_kernel: no atomics.  8 x 2048 x 2048 (bf16, S = 16): 874 us, 216 instructions per
 // 16 channels and step at 47 % issue with 1.7 warps per scheduler; 1985 us with one channel per lane and whole tiles in registers.
 #include <type_traits>
 #include "fwp_scan.cuh"

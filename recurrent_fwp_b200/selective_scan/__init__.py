@@ -16,7 +16,9 @@
   * ``lengths`` (N,) int32 or int64: a padded batch.  Steps at or beyond a sequence's length are not read, give zeros and take no
     gradient; the state is the one after the sequence's own last step.  Values outside 0 ... L count as the nearest of the two.
 
-A call that needs gradients keeps the state before every eighth step for its backward, 4 S / 8 bytes per (step, channel).
+A call that needs gradients keeps the state before every eighth step for its backward, 4 S / 8 bytes per (step, channel).  The backward
+itself takes, while it runs, partial sums for the gradients of B and C: about S * S / 128 bytes per (step, channel), so 2 at 16 states and
+32 at 64, and no less than 8 S bytes per step and group.
 The output's rows lie in the order of x's.  States are float32 and all sums are taken in float32.
 """
 from recurrent_fwp_b200 import _lib
